@@ -257,6 +257,66 @@ INT4MM_API int int4mm_dequantize(int bits, void* w_out, const void* matrix, cons
                       const void* zeros, const void* sparse_mask, int64_t in_size,
                       int64_t out_size, int64_t n_groups, int64_t group_size, void* stream);
 
+/* ---- Products whose rows choose their weights (no counterpart in the reference, whose every product takes one matrix).
+ * All arguments are device pointers, all launches asynchronous on `stream`, and a call uses no memory but its arguments, so
+ * that calls on several streams, and captured ones, need a workspace each and nothing else.  What the
+ * workspace holds before a call does not matter and is undefined after it. */
+
+/* Routing to experts.  logits [tokens, experts], fp16 or fp32; bias fp32 [experts] or NULL; weights fp32 and ids int32
+ * [tokens, top_k], best first:
+ *   p = softmax(logits) (scoring 0) or 1 / (1 + exp(-logits)) (1); an expert whose logit is -inf or NaN is out
+ *   key = logits without a bias, p + bias with one (NaN or -inf: out); the top_k largest keys, ties to the lowest expert
+ *   groups > 1: only experts of the topk_groups best groups of experts / groups neighbours, by their best key (group_score 0)
+ *   or the sum of their two best p (p + bias with a bias; 1), ties to the lowest group
+ *   weights = p, divided by their sum if `renormalize`, times `scale`
+ * p, keys and sums are held in 64 bits, weights rounded once.  Where fewer than top_k experts are left the last slots have
+ * id -1 and weight 0.  experts <= 1024, top_k <= 64, groups <= 64; top_k <= experts / groups * topk_groups. */
+typedef struct int4mm_route_shape {
+    int64_t tokens, experts, top_k, groups, topk_groups;
+    int32_t scoring, group_score, renormalize;
+    int32_t logits_bytes;  /* 2: fp16, 4: fp32 */
+    double scale;
+} int4mm_route_shape;
+INT4MM_API int int4mm_route_experts(void* weights, void* ids, const void* logits, const void* bias,
+                  const int4mm_route_shape* shape, void* stream);
+
+/* The experts' gated feed-forward on packed weights:
+ *   h[t,j,:]  = fp16( silu(x[t,:] @ UP[e][:, :F]) * (x[t,:] @ UP[e][:, F:]) ),   e = ids[t,j]
+ *   outs[t,:] = fp16( sum over j of weights[t,j] * (h[t,j,:] @ DOWN[e]) )         (overwrites outs)
+ * x and outs fp16 [tokens, K], ids int32 and weights fp32 [tokens, top_k].  up_matrix [E, rows, 2 F] and down_matrix [E, rows, K]
+ * hold a packed matrix of in_size K, out_size 2 F and one of F, K per expert in the formats above, scales and zeros [E, groups, 2 F]
+ * and [E, groups, K], masks (16:32: both, else NULL) [E, K / 32, 2 F] and [E, F / 32, K].  A pair whose id is outside 0 ... E - 1
+ * adds nothing (its weight is not looked at); a token without a pair gets 0.  The same expert may be named twice.  Weights are those of
+ * int4mm_dequantize, sums fp32.  Results are a deterministic function of the arguments. */
+typedef struct int4mm_experts_shape {
+    int64_t tokens, top_k, experts;
+    int64_t in_size;       /* K */
+    int64_t width;         /* F */
+    int64_t up_groups;     /* ceil(K / group_size), 1 with a negative group_size */
+    int64_t down_groups;   /* ceil(F / group_size) */
+    int64_t group_size;
+} int4mm_experts_shape;
+INT4MM_API size_t int4mm_experts_workspace_bytes(const int4mm_experts_shape* shape);
+INT4MM_API int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weights, const void* ids,
+                  const void* up_matrix, const void* up_scales, const void* up_zeros, const void* up_mask,
+                  const void* down_matrix, const void* down_scales, const void* down_zeros, const void* down_mask,
+                  const int4mm_experts_shape* shape, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Low-rank adapters of many requests, added onto the output of a projection that they share:
+ *   outs[t,:] = fp16( base[t,:] + scales[a] * (x[t,:] @ down[a]^T) @ up[a] ),   a = ids[t / rows_per_id]
+ * x fp16 [rows, K], base and outs fp16 [rows, S] (outs may be base), down fp16 [adapters, rank, K], up fp16 [adapters, rank, S], scales
+ * fp32 [adapters], ids int32 [ceil(rows / rows_per_id)].  A row whose id is outside 0 ... adapters - 1 keeps its base.  An
+ * adapter of a lower rank has zeros in its last ranks.  K and S multiples of 64, rank 1 ... 512, rows up to 1048560. */
+typedef struct int4mm_adapter_shape {
+    int64_t rows, rows_per_id, adapters, rank;
+    int64_t in_size;       /* K */
+    int64_t out_size;      /* S */
+} int4mm_adapter_shape;
+INT4MM_API size_t int4mm_adapters_workspace_bytes(const int4mm_adapter_shape* shape);
+INT4MM_API int int4mm_low_rank_add(void* outs, const void* base, const void* x, const void* down, const void* up,
+                  const void* scales, const void* ids, const int4mm_adapter_shape* shape,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

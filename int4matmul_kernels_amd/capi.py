@@ -17,6 +17,8 @@ EXPORTS = [
     "int4mm_workspace_bytes", "int4mm_workspace_init", "int4mm_matmul_workspace_bytes", "int4mm_matvec", "int4mm_matmul",
     "int4mm_matvec_overwrite", "int4mm_matvec_static", "int4mm_workspace_status", "int4mm_describe_launch",
     "int4mm_sparse_pack", "int4mm_sparse_pack_checked", "int4mm_dense_pack", "int4mm_unpack", "int4mm_dequantize",
+    "int4mm_route_experts", "int4mm_experts_workspace_bytes", "int4mm_experts_forward",
+    "int4mm_adapters_workspace_bytes", "int4mm_low_rank_add",
 ]
 
 
@@ -30,6 +32,22 @@ class Shape(C.Structure):
     _fields_ = [("batch", C.c_int64), ("seq_len", C.c_int64), ("in_size", C.c_int64),
                 ("out_size", C.c_int64), ("matrix_rows", C.c_int64), ("n_groups", C.c_int64),
                 ("group_size", C.c_int64)]
+
+
+class RouteShape(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("experts", C.c_int64), ("top_k", C.c_int64), ("groups", C.c_int64),
+                ("topk_groups", C.c_int64), ("scoring", C.c_int32), ("group_score", C.c_int32),
+                ("renormalize", C.c_int32), ("logits_bytes", C.c_int32), ("scale", C.c_double)]
+
+
+class ExpertsShape(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("top_k", C.c_int64), ("experts", C.c_int64), ("in_size", C.c_int64),
+                ("width", C.c_int64), ("up_groups", C.c_int64), ("down_groups", C.c_int64), ("group_size", C.c_int64)]
+
+
+class AdapterShape(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("rows_per_id", C.c_int64), ("adapters", C.c_int64), ("rank", C.c_int64),
+                ("in_size", C.c_int64), ("out_size", C.c_int64)]
 
 
 def lib_path() -> str:
@@ -78,6 +96,16 @@ def lib():
     L.int4mm_unpack.argtypes = [C.c_int, vp, vp, vp, vp, i64, i64, vp]
     L.int4mm_dequantize.restype = C.c_int
     L.int4mm_dequantize.argtypes = [C.c_int, vp, vp, vp, vp, vp, i64, i64, i64, i64, vp]
+    L.int4mm_route_experts.restype = C.c_int
+    L.int4mm_route_experts.argtypes = [vp, vp, vp, vp, C.POINTER(RouteShape), vp]
+    L.int4mm_experts_workspace_bytes.restype = sz
+    L.int4mm_experts_workspace_bytes.argtypes = [C.POINTER(ExpertsShape)]
+    L.int4mm_experts_forward.restype = C.c_int
+    L.int4mm_experts_forward.argtypes = [C.c_int] + [vp] * 12 + [C.POINTER(ExpertsShape), vp, sz, vp]
+    L.int4mm_adapters_workspace_bytes.restype = sz
+    L.int4mm_adapters_workspace_bytes.argtypes = [C.POINTER(AdapterShape)]
+    L.int4mm_low_rank_add.restype = C.c_int
+    L.int4mm_low_rank_add.argtypes = [vp] * 7 + [C.POINTER(AdapterShape), vp, sz, vp]
     _LIB = L
     return L
 
@@ -214,3 +242,53 @@ def dequantize(bits, w_out, matrix, scales, zeros, group_size, sparse_mask=None)
     _check(lib().int4mm_dequantize(bits, _ptr(w_out), _ptr(matrix), _ptr(scales), _ptr(zeros),
                                    _ptr(sparse_mask), K, S, G, group_size, _stream()),
            "int4mm_dequantize")
+
+
+def route_experts(weights, ids, logits, scoring="softmax", bias=None, n_groups=1, topk_groups=1, group_score="max",
+                  renormalize=True, scale=1.0):
+    """``logits`` [tokens, experts] to ``weights`` (fp32) and ``ids`` (int32), both [tokens, top_k]"""
+    T, E = logits.shape
+    sh = RouteShape(T, E, ids.shape[-1], n_groups, topk_groups, ("softmax", "sigmoid").index(scoring), ("max", "top2").index(group_score),
+                    int(renormalize), logits.element_size(), scale)
+    _check(lib().int4mm_route_experts(_ptr(weights), _ptr(ids), _ptr(logits), _ptr(bias), C.byref(sh), _stream()),
+           "int4mm_route_experts")
+
+
+def experts_shape(tokens, top_k, experts, in_size, width, group_size):
+    up, down = (1 if group_size < 0 else -(-k // group_size) for k in (in_size, width))
+    return ExpertsShape(tokens, top_k, experts, in_size, width, up, down, group_size)
+
+
+def new_experts_workspace(tokens, top_k, experts, in_size, width, group_size=128, device="cuda"):
+    import torch
+    sh = experts_shape(tokens, top_k, experts, in_size, width, group_size)
+    return torch.empty(lib().int4mm_experts_workspace_bytes(C.byref(sh)), dtype=torch.uint8, device=device)
+
+
+def experts_forward(bits, outs, x, weights, ids, up, down, group_size, workspace=None):
+    """``up`` and ``down``: (matrix, scales, zeros, mask or None) of all experts"""
+    T, K = x.shape
+    E, _, columns = up[0].shape
+    sh = experts_shape(T, ids.shape[-1], E, K, columns // 2, group_size)
+    nws = 0 if workspace is None else workspace.numel()
+    _check(lib().int4mm_experts_forward(bits, _ptr(outs), _ptr(x), _ptr(weights), _ptr(ids), *map(_ptr, up), *map(_ptr, down),
+                                        C.byref(sh), _ptr(workspace), nws, _stream()), "int4mm_experts_forward")
+
+
+def _adapter_shape(rows, rows_per_id, down, up):
+    n, rank, K = down.shape
+    return AdapterShape(rows, rows_per_id, n, rank, K, up.shape[-1])
+
+
+def new_adapters_workspace(rows, rows_per_id, down, up):
+    import torch
+    sh = _adapter_shape(rows, rows_per_id, down, up)
+    return torch.empty(lib().int4mm_adapters_workspace_bytes(C.byref(sh)), dtype=torch.uint8, device=down.device)
+
+
+def low_rank_add(outs, base, x, down, up, scales, ids, rows_per_id=1, workspace=None):
+    """``outs = base + scales[a] * (x @ down[a].T) @ up[a]`` row by row, ``a = ids[row // rows_per_id]``"""
+    sh = _adapter_shape(x.shape[0], rows_per_id, down, up)
+    nws = 0 if workspace is None else workspace.numel()
+    _check(lib().int4mm_low_rank_add(_ptr(outs), _ptr(base), _ptr(x), _ptr(down), _ptr(up), _ptr(scales), _ptr(ids),
+                                     C.byref(sh), _ptr(workspace), nws, _stream()), "int4mm_low_rank_add")

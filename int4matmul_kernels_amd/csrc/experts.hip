@@ -1,0 +1,391 @@
+// The experts' gated feed-forward on packed weights: of tokens x [T, K] with the experts ids [T, k] and their weights [T, k]
+//     h[t, j, :] = silu(x[t] up_e[:, :F]) * (x[t] up_e[:, F:]),   outs[t, :] = fp16( sum_j weights[t, j] * (h[t, j] down_e) ),
+// e = ids[t, j]; a pair whose id is outside 0 ... E - 1 has no expert and adds nothing.  Every weight is dequantised as the
+// products of the linear layers do it, fp16(fp16(q - z) s) or the exponent mode's fma, sums are fp32, h is rounded to fp16 (it
+// is an operand of the matrix instructions), and so is the result.
+//
+//   plan_kernel     pairs in the order of their experts, stable: where each expert's begin, the pairs, each pair's place
+//   rows_kernel     a product of the pairs of one expert, up to 16 MT at a time, with a strip of 64 columns
+//   combine_kernel  the weighted sum of a token's k results, fp32
+//
+// rows_kernel is bound by reading the packed weights.  The waves of a workgroup share K out, so nothing is shared through LDS
+// in the loop: a lane loads 16 bytes of packed words, four neighbouring columns of the packed row that holds its 8 k, and each
+// word is after its decode the operand of one v_mfma_f32_16x16x32_f16 whose columns are every fourth of the strip; the states'
+// operands come straight from global memory, where the waves of all strips find them in the L2.  The partial sums meet in LDS.
+#include "decode.h"
+
+#include <algorithm>
+
+namespace i4 {
+
+struct ExpertsArgs {
+    const h16* x;                  // source rows
+    const uint32_t* matrix;
+    const uint32_t* mask;
+    const h16* scales;
+    const h16* zeros;
+    const int* offsets;            // [E + 1]: an expert's pairs among the ordered ones
+    const int* order;              // [P]: pair of each place
+    h16* h;                        // up: [P, F] by place
+    float* part;                   // down: [P, S] by place
+    int64_t matrix_stride, mask_stride, scale_stride;   // elements from an expert to the next
+    int experts, top_k, K, S;      // S: columns of the matrix (up: 2 F)
+    int group_units, strips;       // strips: of 64 columns
+};
+
+template <int BITS, bool SPARSE> struct RowsFmt;       // packed rows of a 32-row block, 16-byte loads of a lane per block
+template <> struct RowsFmt<4, false> { static constexpr int ROWS = 4, LOADS = 1; };
+template <> struct RowsFmt<3, false> { static constexpr int ROWS = 3, LOADS = 2; };
+template <> struct RowsFmt<2, false> { static constexpr int ROWS = 2, LOADS = 1; };
+template <> struct RowsFmt<4, true> { static constexpr int ROWS = 2, LOADS = 3; };
+
+// ---- pairs in the order of their experts: workgroup e finds how many pairs belong to lower experts, and places its own.  Each
+// of the 16 waves takes a share of the pairs, twice: counting, then placing; no atomics, the order is that of the pairs.
+__global__ __launch_bounds__(1024) void plan_kernel(const int* ids, int* offsets, int* order, int* place, int pairs, int experts) {
+    __shared__ int of_wave[16], lower;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), e = blockIdx.x;
+    const int share = ((pairs + 15) / 16 + 63) & ~63, from = min(wave * share, pairs), to = min(from + share, pairs);
+    if (t == 0) lower = 0;
+    __syncthreads();
+    int mine = 0, below = 0;
+#pragma unroll 4
+    for (int i = from; i < to; i += 64) {
+        const int id = i + lane < to ? ids[i + lane] : -1;
+        mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(id == e));
+        below += __builtin_popcountll(__builtin_amdgcn_ballot_w64(id >= 0 && id < e));
+    }
+    if (lane == 0) {
+        of_wave[wave] = mine;
+        atomicAdd(&lower, below);                     // (whole numbers: any order)
+    }
+    __syncthreads();
+    int at = lower, all = 0;
+    for (int w = 0; w < 16; ++w) {
+        at += w < wave ? of_wave[w] : 0;
+        all += of_wave[w];
+    }
+    if (t == 0) {
+        offsets[e] = lower;
+        if (e == experts - 1) offsets[experts] = lower + all;
+    }
+#pragma unroll 4
+    for (int i = from; i < to; i += 64) {
+        const int p = i + lane, id = p < to ? ids[p] : -1;
+        const uint64_t in = __builtin_amdgcn_ballot_w64(id == e);
+        if (id == e) {
+            const int where = at + __builtin_popcountll(in & ((1ull << lane) - 1));
+            order[where] = p;
+            place[p] = where;
+        } else if (e == 0 && p < to && (id < 0 || id >= experts)) {
+            place[p] = -1;
+        }
+        at += __builtin_popcountll(in);
+    }
+}
+
+// which expert's rows, and the first of them, is block `want` of blocks of `height` pairs each?  False: there are fewer blocks
+__device__ __forceinline__ bool find_block(const int* offsets, int experts, int height, int want, int lane, int& expert, int& first, int& count) {
+    for (int e0 = 0; e0 < experts; e0 += 64) {
+        const int e = e0 + lane;
+        const int a = offsets[min(e, experts)], b = offsets[min(e + 1, experts)];
+        const int blocks = (b - a + height - 1) / height;
+        int upto = blocks;                            // blocks of this lane's and the lower lanes' experts
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int o = __shfl_up(upto, d);
+            upto += lane >= d ? o : 0;
+        }
+        const uint64_t beyond = __builtin_amdgcn_ballot_w64(upto > want);
+        if (beyond) {
+            const int l = __builtin_ctzll(beyond);
+            expert = e0 + l;
+            const int nth = want - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(blocks, l));
+            const int from = __builtin_amdgcn_readlane(a, l), to = __builtin_amdgcn_readlane(b, l);
+            first = from + nth * height;
+            count = min(height, to - first);
+            return true;
+        }
+        want -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
+// ---- a product of up to 16 MT pairs of one expert with 64 columns.  UP: 32 columns of the gate and the same 32 of the other
+// half; the source row of a pair is its token's, the result h.  Else: 64 columns, source and result by place.
+template <int BITS, bool SPARSE, int MT, int WAVES, bool UP>
+__global__ __launch_bounds__(64 * WAVES) void rows_kernel(ExpertsArgs a) {
+    using F = RowsFmt<BITS, SPARSE>;
+    constexpr int HEIGHT = 16 * MT;
+    __shared__ __attribute__((aligned(16))) float red[WAVES * HEIGHT * 64];
+    __shared__ __attribute__((aligned(16))) uint32_t lut[SPARSE ? SPARSE_LUT_WORDS : 4];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int n = lane & 15, q = lane >> 4;
+    int expert, first, count;
+    if (!find_block(a.offsets, a.experts, HEIGHT, blockIdx.x / a.strips, lane, expert, first, count)) return;
+    const int strip = blockIdx.x % a.strips;
+    if constexpr (SPARSE) {
+        for (int e = t; e < 256; e += 64 * WAVES) {
+            uint32_t v[8];
+            sparse_lut_entry(e, v);
+            *reinterpret_cast<u32x4*>(lut + e * 8) = u32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<u32x4*>(lut + e * 8 + 4) = u32x4{v[4], v[5], v[6], v[7]};
+        }
+        __syncthreads();
+    }
+    const int half = a.S / 2;
+    // lane n's four columns of the strip
+    const int col = UP ? (n < 8 ? 0 : half - 32) + 32 * strip + 4 * n : 64 * strip + 4 * n;
+    const h16* xrow[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int at = first + min(16 * m + n, count - 1);              // (rows beyond the last repeat it and are not written)
+        xrow[m] = a.x + (int64_t)(UP ? a.order[at] / a.top_k : at) * a.K + 8 * q;
+    }
+    const uint32_t* const matrix = a.matrix + expert * a.matrix_stride;
+    const uint32_t* const mask = SPARSE ? a.mask + expert * a.mask_stride : nullptr;
+    const h16* const scales = a.scales + expert * a.scale_stride + col;
+    const h16* const zeros = a.zeros + expert * a.scale_stride + col;
+
+    f32x4 acc[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    struct Unit {                                     // 64 k
+        u32x4 w[2][F::LOADS];
+        u32x4 x[2][MT];
+        u32x2 s, z;
+    };
+    const uint32_t row0 = BITS == 4 && !SPARSE ? q : BITS == 2 ? q >> 1 : BITS == 3 ? (q > 0 ? q - 1 : 0) : 0;
+    auto load = [&](Unit& u, int unit) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const uint32_t* const blk = matrix + (int64_t)(2 * unit + b) * F::ROWS * a.S + col;
+            u.w[b][0] = *reinterpret_cast<const u32x4*>(blk + (uint32_t)(row0 * a.S));
+            if constexpr (BITS == 3) u.w[b][1] = *reinterpret_cast<const u32x4*>(blk + (uint32_t)(min((int)row0 + 1, 2) * a.S));
+            if constexpr (SPARSE) {
+                u.w[b][1] = *reinterpret_cast<const u32x4*>(blk + a.S);
+                u.w[b][2] = *reinterpret_cast<const u32x4*>(mask + (int64_t)(2 * unit + b) * a.S + col);
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) u.x[b][m] = *reinterpret_cast<const u32x4*>(xrow[m] + 64 * unit + 32 * b);
+        }
+        const int64_t g = (int64_t)(unit / a.group_units) * a.S;
+        u.s = *reinterpret_cast<const u32x2*>(scales + g);
+        u.z = *reinterpret_cast<const u32x2*>(zeros + g);
+    };
+    auto multiply = [&](auto mode, const Unit& u) __attribute__((always_inline)) {
+        Coef<BITS, decltype(mode)::value> co[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t sel = (j & 1) ? 0x03020302u : 0x01000100u;
+            co[j].set(as_h2(__builtin_amdgcn_perm(u.s[j >> 1], u.s[j >> 1], sel)), as_h2(__builtin_amdgcn_perm(u.z[j >> 1], u.z[j >> 1], sel)));
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h16x8 w;
+                if constexpr (SPARSE) {
+                    const uint32_t m = u.w[b][2][j], m8 = (m >> (8 * q)) & 0xFFu;
+                    const uint32_t skip = __builtin_popcount(m & ((1u << (8 * q)) - 1u));
+                    const uint64_t st = ((uint64_t)u.w[b][1][j] << 32) | u.w[b][0][j];
+                    w = dequant_chunk_sparse((uint32_t)((st >> (2 * skip)) >> (2 * skip)), m8, lut, co[j]);
+                } else if constexpr (BITS == 4) {
+                    w = dequant_chunk<4>(u.w[b][0][j], co[j]);
+                } else if constexpr (BITS == 2) {
+                    w = dequant_chunk<2>(u.w[b][0][j] >> (16 * (q & 1)), co[j]);
+                } else {
+                    // bits 24 q ... 24 q + 23 of the 96
+                    const uint32_t lo = u.w[b][0][j], hi = u.w[b][1][j];
+                    w = dequant_chunk<3>(q == 0 ? lo : q == 1 ? __builtin_amdgcn_alignbit(hi, lo, 24) : q == 2 ? __builtin_amdgcn_alignbit(hi, lo, 16) : hi >> 8, co[j]);
+                }
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<h16x8>(u.x[b][m]), w, acc[m][j], 0, 0, 0);
+            }
+    };
+    const int units = a.K / 64, u0 = units * wave / WAVES, u1 = units * (wave + 1) / WAVES;
+    auto take = [&](const Unit& now) __attribute__((always_inline)) {
+        // a negative or NaN scale anywhere in the wave: the decode that serves either mode
+        if (BITS == 4 && __builtin_amdgcn_ballot_w64(((now.s[0] | now.s[1]) & 0x80008000u) != 0) != 0) multiply(std::bool_constant<BITS == 4>{}, now);
+        else multiply(std::false_type{}, now);
+    };
+    Unit ua, ub;
+    if (u0 < u1) load(ua, u0);
+    for (int i = u0; i < u1; i += 2) {
+        if (i + 1 < u1) load(ub, i + 1);
+        take(ua);
+        if (i + 2 < u1) load(ua, i + 2);
+        if (i + 1 < u1) take(ub);
+    }
+    // register r of tile (m, j): row 16 m + 4 q + r, column 4 n + j of the strip
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            *reinterpret_cast<f32x4*>(red + (wave * HEIGHT + 16 * m + 4 * q + r) * 64 + 4 * n) = f32x4{acc[m][0][r], acc[m][1][r], acc[m][2][r], acc[m][3][r]};
+    __syncthreads();
+    auto total = [&](int row, int c) __attribute__((always_inline)) {
+        f32x4 s = *reinterpret_cast<const f32x4*>(red + row * 64 + c);
+        for (int w = 1; w < WAVES; ++w) s += *reinterpret_cast<const f32x4*>(red + (w * HEIGHT + row) * 64 + c);
+        return s;
+    };
+    constexpr int QUADS = UP ? 8 : 16;                // quadruples of results in a row
+    for (int i = t; i < HEIGHT * QUADS; i += 64 * WAVES) {
+        const int row = i / QUADS, c = i % QUADS * 4;
+        if (row >= count) break;
+        if constexpr (UP) {
+            const f32x4 gate = total(row, c), up = total(row, c + 32);
+            h16x4 o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = (h16)(gate[j] / (1.f + __expf(-gate[j])) * up[j]);
+            *reinterpret_cast<h16x4*>(a.h + (int64_t)(first + row) * half + 32 * strip + c) = o;
+        } else {
+            *reinterpret_cast<f32x4*>(a.part + (int64_t)(first + row) * a.S + 64 * strip + c) = total(row, c);
+        }
+    }
+}
+
+// outs[t, :] = sum over j of weights[t, j] part[place[t, j], :]; a thread takes four columns
+__global__ __launch_bounds__(256) void combine_kernel(h16* outs, const float* part, const float* weights, const int* place, int top_k, int S, int parts) {
+    const int64_t t = blockIdx.x / parts;
+    const int c = ((int)(blockIdx.x % parts) * 256 + threadIdx.x) * 4;
+    if (c >= S) return;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < top_k; ++j) {
+        const int p = place[t * top_k + j];
+        if (p >= 0) sum += weights[t * top_k + j] * *reinterpret_cast<const f32x4*>(part + (int64_t)p * S + c);
+    }
+    *reinterpret_cast<h16x4*>(outs + t * S + c) = h16x4{(h16)sum[0], (h16)sum[1], (h16)sum[2], (h16)sum[3]};
+}
+
+template <int BITS, bool SPARSE, bool UP>
+static void launch_rows(ExpertsArgs a, int mt, int64_t pairs, hipStream_t st) {
+    a.strips = a.S / 64;
+    const int64_t height = 16 * mt, blocks = std::min<int64_t>(pairs, a.experts + pairs / height);
+    const dim3 grid((unsigned)(blocks * a.strips));
+    if (mt == 1) hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 1, 8, UP>), grid, dim3(512), 0, st, a);
+    else if (mt == 2) hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 2, 4, UP>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 4, 4, UP>), grid, dim3(256), 0, st, a);
+}
+
+template <bool UP>
+static void rows_product(int bits, const ExpertsArgs& a, int mt, int64_t pairs, hipStream_t st) {
+    if (a.mask) launch_rows<4, true, UP>(a, mt, pairs, st);
+    else if (bits == 4) launch_rows<4, false, UP>(a, mt, pairs, st);
+    else if (bits == 3) launch_rows<3, false, UP>(a, mt, pairs, st);
+    else launch_rows<2, false, UP>(a, mt, pairs, st);
+}
+
+static int check_experts(int bits, const int4mm_experts_shape* sh, bool sparse) {
+    if (sh == nullptr) return INT4MM_ERR_NULL;
+    if (bits != 4 && bits != 3 && bits != 2) return INT4MM_ERR_BITS;
+    if (sparse && bits != 4) return INT4MM_ERR_SPARSE_BITS;
+    const int64_t limit = (int64_t)1 << 31, K = sh->in_size, F = sh->width, g = sh->group_size;
+    if (sh->tokens < 0 || sh->top_k < 1 || sh->experts < 1 || sh->experts > 65536 || K <= 0 || F <= 0 || K % 64 != 0 || F % 64 != 0) return INT4MM_ERR_SHAPE;
+    if (g == 0 || (g > 0 && g % 64 != 0)) return INT4MM_ERR_GROUP;
+    const int64_t up_groups = g < 0 ? 1 : (K + g - 1) / g, down_groups = g < 0 ? 1 : (F + g - 1) / g;
+    if (sh->up_groups != up_groups || sh->down_groups != down_groups) return INT4MM_ERR_SHAPE;
+    // (a row of a block is addressed with 32 bits from the block's first, and a grid has so many rows)
+    if (K > limit / 64 || F > limit / 64 || K * F >= limit * 16) return INT4MM_ERR_SHAPE;
+    // (grids of one dimension: a workgroup per 16 pairs or expert and 64 columns)
+    if (sh->top_k > 1024 || sh->tokens > limit || (sh->tokens * sh->top_k / 16 + sh->experts) * (std::max(K, 2 * F) / 64) >= limit ||
+        sh->tokens * sh->top_k >= limit / 2)
+        return INT4MM_ERR_SHAPE;
+    return INT4MM_OK;
+}
+
+struct ExpertsParts { size_t offsets, order, place, h, part, total; };
+static ExpertsParts experts_parts(const int4mm_experts_shape& sh) {
+    const size_t pairs = (size_t)(sh.tokens * sh.top_k);
+    auto round = [](size_t n) { return (n + 255) & ~size_t(255); };
+    ExpertsParts p;
+    p.offsets = 0;
+    p.order = p.offsets + round(4 * (size_t)(sh.experts + 1));
+    p.place = p.order + round(4 * pairs);
+    p.h = p.place + round(4 * pairs);
+    p.part = p.h + round(2 * pairs * (size_t)sh.width);
+    p.total = p.part + round(4 * pairs * (size_t)sh.in_size);
+    return p;
+}
+
+}  // namespace i4
+
+using namespace i4;
+
+extern "C" {
+
+size_t int4mm_experts_workspace_bytes(const int4mm_experts_shape* sh) {
+    if (sh == nullptr || sh->tokens <= 0 || sh->top_k <= 0 || sh->experts <= 0 || sh->width <= 0 || sh->in_size <= 0) return 0;
+    return experts_parts(*sh).total;
+}
+
+int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weights, const void* ids, const void* up_matrix,
+                           const void* up_scales, const void* up_zeros, const void* up_mask, const void* down_matrix,
+                           const void* down_scales, const void* down_zeros, const void* down_mask, const int4mm_experts_shape* sh,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+    const bool sparse = up_mask != nullptr || down_mask != nullptr;
+    if (const int rc = check_experts(bits, sh, sparse)) return rc;
+    if (sh->tokens == 0) return INT4MM_OK;
+    if (!outs || !x || !weights || !ids || !up_matrix || !up_scales || !up_zeros || !down_matrix || !down_scales || !down_zeros ||
+        (sparse && (!up_mask || !down_mask)))
+        return INT4MM_ERR_NULL;
+    const void* aligned[] = {outs, x, up_matrix, up_scales, up_zeros, up_mask, down_matrix, down_scales, down_zeros, down_mask, workspace};
+    for (const void* ptr : aligned)
+        if (reinterpret_cast<uintptr_t>(ptr) & 15) return INT4MM_ERR_ALIGN;
+    if ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(ids)) & 3) return INT4MM_ERR_ALIGN;
+    const ExpertsParts parts = experts_parts(*sh);
+    if (workspace == nullptr || workspace_bytes < parts.total) return INT4MM_ERR_WORKSPACE;
+    char* const ws = static_cast<char*>(workspace);
+    const int64_t pairs = sh->tokens * sh->top_k, K = sh->in_size, F = sh->width;
+    const int E = (int)sh->experts;
+    hipStream_t st = (hipStream_t)stream;
+    int* const place = reinterpret_cast<int*>(ws + parts.place);
+    ExpertsArgs a;
+    a.offsets = reinterpret_cast<int*>(ws + parts.offsets);
+    a.order = reinterpret_cast<int*>(ws + parts.order);
+    a.h = reinterpret_cast<h16*>(ws + parts.h);
+    a.part = reinterpret_cast<float*>(ws + parts.part);
+    a.experts = E;
+    a.top_k = (int)sh->top_k;
+    a.group_units = (int)(sh->group_size < 0 ? ONE_GROUP / 64 : sh->group_size / 64);
+    hipLaunchKernelGGL(plan_kernel, dim3(E), dim3(1024), 0, st, static_cast<const int*>(ids), const_cast<int*>(a.offsets),
+                           const_cast<int*>(a.order), place, (int)pairs, E);
+    if (const int rc = check_launch("experts_forward")) return rc;
+    // pairs per expert, if all are asked alike
+    const int64_t mean = pairs / E;
+    const int mt = mean <= 8 ? 1 : mean <= 24 ? 2 : 4;
+    auto rows_of = [&](int64_t k) { return sparse ? k / 16 : k * bits / 32; };
+    a.x = static_cast<const h16*>(x);
+    a.matrix = static_cast<const uint32_t*>(up_matrix);
+    a.mask = static_cast<const uint32_t*>(up_mask);
+    a.scales = static_cast<const h16*>(up_scales);
+    a.zeros = static_cast<const h16*>(up_zeros);
+    a.K = (int)K;
+    a.S = (int)(2 * F);
+    a.matrix_stride = rows_of(K) * 2 * F;
+    a.mask_stride = K / 32 * 2 * F;
+    a.scale_stride = sh->up_groups * 2 * F;
+    rows_product<true>(bits, a, mt, pairs, st);
+    if (const int rc = check_launch("experts_forward")) return rc;
+    a.x = a.h;
+    a.matrix = static_cast<const uint32_t*>(down_matrix);
+    a.mask = static_cast<const uint32_t*>(down_mask);
+    a.scales = static_cast<const h16*>(down_scales);
+    a.zeros = static_cast<const h16*>(down_zeros);
+    a.K = (int)F;
+    a.S = (int)K;
+    a.matrix_stride = rows_of(F) * K;
+    a.mask_stride = F / 32 * K;
+    a.scale_stride = sh->down_groups * K;
+    rows_product<false>(bits, a, mt, pairs, st);
+    if (const int rc = check_launch("experts_forward")) return rc;
+    const int columns = (int)((K / 4 + 255) / 256);
+    hipLaunchKernelGGL(combine_kernel, dim3((unsigned)(sh->tokens * columns)), dim3(256), 0, st, static_cast<h16*>(outs), a.part, static_cast<const float*>(weights), place,
+                           a.top_k, (int)K, columns);
+    return check_launch("experts_forward");
+}
+
+}  // extern "C"

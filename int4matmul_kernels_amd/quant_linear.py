@@ -102,7 +102,11 @@ class QuantLinear(torch.nn.Module):
         return m
 
     # ------------------------------------------------------------------ forward
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, adapters: Optional[torch.nn.Module] = None, adapter_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``x`` ``[..., in_features]``.  With ``adapters`` (a ``LowRankAdapters``) every row's own low-rank term is added:
+        ``adapter_ids`` (int32) are ``x``'s leading sizes, one or more of them"""
+        if (adapters is None) != (adapter_ids is None):
+            raise ValueError("adapters and adapter_ids come together")
         # (the buffers straight from their dict: nn.Module's attribute look-up takes 0.3 us for each of the five)
         b = self._buffers
         try:
@@ -114,6 +118,8 @@ class QuantLinear(torch.nn.Module):
                                                 scales, zeros, self.group_size, mask)
         if flat:
             y = y.reshape(*x.shape[:-1], self.out_features)
+        if adapters is not None:
+            y = adapters(y, x, adapter_ids, outs=y)
         return y if bias is None else y + bias
 
     def dequantized_weight(self) -> torch.Tensor:
