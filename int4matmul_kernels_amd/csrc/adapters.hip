@@ -13,7 +13,6 @@
 #include "common.h"
 
 #include <algorithm>
-#include <climits>
 
 namespace i4 {
 
@@ -34,46 +33,47 @@ struct AdapterArgs {
     uint32_t id_magic;
     int adapters, rank, K, S;
     int ksplit, units_per_split;                      // units of 64 k
-    int deal;                                         // workgroup z takes every deal-th of a tile's distinct adapters
-    int columns;                                      // expand: columns per workgroup
+    // the distinct adapters of a tile are dealt to `deal` workgroups (a power of two) by the first row of each; deal_rows: every
+    // deal-th bit from bit 0
+    int deal;
+    uint64_t deal_rows;
+    int strips;                                       // expand: of 256 columns, per workgroup
 };
-
-template <int CTRL>
-__device__ __forceinline__ int dpp_min(int v) {
-    return min(v, __builtin_amdgcn_update_dpp(INT_MAX, v, CTRL, 0xF, 0xF, false));
-}
-// the smallest of the values in a row of 16 lanes, the same in all rows
-__device__ __forceinline__ int row_min(int v) {
-    v = dpp_min<0xB1>(v);
-    v = dpp_min<0x4E>(v);
-    v = dpp_min<0x141>(v);
-    v = dpp_min<0x140>(v);
-    return __builtin_amdgcn_readfirstlane(v);
-}
 
 // (rows < 2^22: check_adapters)
 __device__ __forceinline__ int id_of(const AdapterArgs& a, int64_t row) { return magic_div((int)row, a.rows_per_id, a.id_magic); }
 
-// ids of the tile's rows: lane l holds those of rows l % 16 + 16 m; -1: no adapter
-template <int MT>
-__device__ __forceinline__ void tile_ids(int (&id)[MT], const AdapterArgs& a, int64_t row0, int lane) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int64_t row = row0 + 16 * m + (lane & 15);
-        int v = row < a.rows ? a.ids[id_of(a, row)] : -1;
-        id[m] = v >= 0 && v < a.adapters ? v : -1;
+// The adapters of a tile of up to 64 neighbouring rows: lane i holds row i's id, -1 without one.  Rows are masks of 64 bits.
+struct Tile {
+    int id;
+    uint64_t there;                                   // rows that exist
+    uint64_t with;                                    // rows that have an adapter
+    uint64_t dealt;                                   // rows whose adapters are this workgroup's, where they are the first of theirs
+};
+__device__ __forceinline__ Tile tile_of(const AdapterArgs& a, int64_t row0, int height, int lane, int deal) {
+    Tile t;
+    const int64_t row = row0 + lane;
+    const bool there = lane < height && row < a.rows;
+    const int v = there ? a.ids[id_of(a, row)] : -1;
+    t.id = v >= 0 && v < a.adapters ? v : -1;
+    t.there = __builtin_amdgcn_ballot_w64(there);
+    t.with = __builtin_amdgcn_ballot_w64(t.id >= 0);
+    t.dealt = a.deal_rows << deal;
+    return t;
+}
+// calls f(adapter, its rows) for each of this workgroup's adapters
+template <class F>
+__device__ __forceinline__ void each_adapter(const Tile& t, F f) {
+    uint64_t left = t.with & t.dealt;
+    while (left) {
+        const int row = __builtin_ctzll(left), adapter = __builtin_amdgcn_readlane(t.id, row);
+        const uint64_t rows = __builtin_amdgcn_ballot_w64(t.id == adapter);
+        left &= ~rows;
+        if (__builtin_ctzll(rows) == row) f(adapter, rows);
     }
 }
-// the smallest id above `last` in the tile (INT_MAX: none)
-template <int MT>
-__device__ __forceinline__ int next_id(const int (&id)[MT], int last) {
-    int v = INT_MAX;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) v = min(v, id[m] > last ? id[m] : INT_MAX);
-    return row_min(v);
-}
 
-// 16 MT rows, 16 NT ranks from rank0 = 16 NT blockIdx.z', a share of K; the four waves share it out by units of 64 k
+// 16 MT rows, 16 NT ranks, a share of K; the four waves share it out by units of 64 k
 template <int MT, int NT>
 __global__ __launch_bounds__(256) void shrink_kernel(AdapterArgs a) {
     __shared__ __attribute__((aligned(16))) float red[4 * 16 * MT * 16 * NT];
@@ -83,43 +83,38 @@ __global__ __launch_bounds__(256) void shrink_kernel(AdapterArgs a) {
     const int deal = blockIdx.z % a.deal, rank0 = blockIdx.z / a.deal * (16 * NT);
     const int units = a.K / 64, u0 = blockIdx.x * a.units_per_split, u1 = min(u0 + a.units_per_split, units);
     const uint32_t pitch = 2u * (uint32_t)a.K;
-    int id[MT];
-    tile_ids<MT>(id, a, row0, lane);
+    const Tile tile = tile_of(a, row0, 16 * MT, lane, deal);
     const int rows_here = (int)min((int64_t)(16 * MT), a.rows - row0), ranks_here = min(16 * NT, a.rank - rank0);
     const __amdgpu_buffer_rsrc_t x_rsrc =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<h16*>(a.x) + row0 * a.K, 0, (int)(rows_here * pitch), AD_RSRC);
-    // lane group q takes k = 16 q ... 16 q + 15 of a unit in two steps: 128 bytes of a row per step pair
+    // lane group q takes k = 16 q ... 16 q + 15 of a unit in two steps: 128 bytes of a row per pair of steps
     const uint32_t at = (uint32_t)n * pitch + 32u * q;
 
-    int last = -1;
-    for (int index = 0;; ++index) {
-        const int cur = next_id<MT>(id, last);
-        if (cur == INT_MAX) break;
-        last = cur;
-        if (index % a.deal != deal) continue;
+    each_adapter(tile, [&](int cur, uint64_t rows) __attribute__((always_inline)) {
         const __amdgpu_buffer_rsrc_t w_rsrc = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<h16*>(a.down) + ((int64_t)cur * a.rank + rank0) * a.K, 0, (int)(ranks_here * pitch), AD_RSRC);
-        uint32_t xo[MT];
+        uint32_t xo[MT];                              // (only this adapter's rows are read)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) xo[m] = (at + 16u * m * pitch) | (id[m] == cur ? 0u : AD_BEYOND);
+        for (int m = 0; m < MT; ++m) xo[m] = (at + 16u * m * pitch) | ((rows >> (16 * m + n)) & 1 ? 0u : AD_BEYOND);
         f32x4 acc[MT][NT];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-        for (int u = u0 + wave; u < u1; u += 4) {
-            u32x4 xv[2][MT], wv[2][NT];
+        // (two units a trip, the second one perhaps beyond the share: it reads as 0)
+        for (int u = u0 + wave; u < u1; u += 8) {
+            u32x4 xv[4][MT], wv[4][NT];
+            const uint32_t beyond = u + 4 < u1 ? 0u : AD_BEYOND;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
+            for (int s = 0; s < 4; ++s) {
+                const uint32_t off = 128u * (u + (s >> 1) * 4) + 16u * (s & 1), past = s >> 1 ? beyond : 0u;
 #pragma unroll
-                for (int m = 0; m < MT; ++m) xv[s][m] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, xo[m], 128u * u + 16u * s, 0);
+                for (int m = 0; m < MT; ++m) xv[s][m] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, xo[m] | past, off, 0);
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    wv[s][t] = __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, at + 16u * t * pitch, 128u * u + 16u * s, 0);
+                for (int t = 0; t < NT; ++t) wv[s][t] = __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, (at + 16u * t * pitch) | past, off, 0);
             }
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (int s = 0; s < 4; ++s)
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -138,16 +133,19 @@ __global__ __launch_bounds__(256) void shrink_kernel(AdapterArgs a) {
         for (int i = 0; i < MT * NT; ++i) {
             const int e = i * 256 + threadIdx.x, row = e / (16 * NT), rank = e % (16 * NT);
             const float sum = (red[e] + red[e + 256 * MT * NT]) + (red[e + 512 * MT * NT] + red[e + 768 * MT * NT]);
-            const int64_t at_row = row0 + row;
-            if (at_row < a.rows && rank < ranks_here && a.ids[id_of(a, at_row)] == cur)
-                a.part[((int64_t)blockIdx.x * a.rows + at_row) * a.rank + rank0 + rank] = sum;
+            if (((rows >> row) & 1) && rank < ranks_here)
+                a.part[((int64_t)blockIdx.x * a.rows + row0 + row) * a.rank + rank0 + rank] = sum;
         }
         __syncthreads();
-    }
+    });
 }
 
-// 16 MT rows, `columns` columns: four waves of 64 columns at a time
-template <int MT>
+template <int CTRL>
+__device__ __forceinline__ float dpp_fmax(float v) { return fmaxf(v, dpp_f32<CTRL>(v)); }
+
+// 16 MT rows, `strips` times 256 columns: four waves of 64 columns, tile j of a wave takes columns 4 n + j.  LONG: more than 64
+// ranks.  The first adapter's first PRE times 32 ranks and base are asked for a strip ahead.
+template <int MT, bool LONG, int PRE>
 __global__ __launch_bounds__(256) void expand_kernel(AdapterArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -158,82 +156,121 @@ __global__ __launch_bounds__(256) void expand_kernel(AdapterArgs a) {
     h16* const high = reinterpret_cast<h16*>(lds);
     h16* const low = high + 16 * MT * pitch;
     float* const unscale = reinterpret_cast<float*>(low + 16 * MT * pitch);
-    int id[MT];
-    tile_ids<MT>(id, a, row0, lane);
+    const Tile tile = tile_of(a, row0, 16 * MT, lane, deal);
 
-    // ---- h of the tile's rows: a wave takes a row at a time
-    for (int row = wave; row < 16 * MT; row += 4) {
-        const int64_t at_row = row0 + row;
-        const int of = at_row < a.rows ? a.ids[id_of(a, at_row)] : -1;
-        const bool there = of >= 0 && of < a.adapters;
-        const float scale = there ? a.scales[of] : 0.f;
-        float most = 0.f;
-        float h[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            h[i] = 0.f;
-            if (64 * i < a.rank) {
-                const int rank = 64 * i + lane;
-                if (there && rank < a.rank) {
-                    float sum = 0.f;
-                    for (int ks = 0; ks < a.ksplit; ++ks) sum += a.part[((int64_t)ks * a.rows + at_row) * a.rank + rank];
-                    h[i] = sum * scale;
-                }
-                most = fmaxf(most, fabsf(h[i]));
-            }
-        }
-#pragma unroll
-        for (int d = 1; d < WAVE; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-        // most = f 2^e, f in [0.5, 1): times 2^(10 - e)
-        int e = 10;
-        if (most > 0.f && most < INFINITY) e = __builtin_amdgcn_frexp_expf(most);
-        e = max(e, -100);
-        const float by = __builtin_ldexpf(1.f, 10 - e);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int rank = 64 * i + lane;
-            if (64 * i < a.rank && rank < chunks * 32) {
-                const float v = h[i] * by;
-                const h16 hi = (h16)v;
-                // (an infinity or NaN is in the high part alone)
-                const float rest = fabsf(v) < 65504.f ? v - (float)hi : 0.f;
-                high[row * pitch + rank] = hi;
-                low[row * pitch + rank] = (h16)rest;
-            }
-        }
-        if (lane == 0) unscale[row] = __builtin_ldexpf(1.f, e - 10);
-    }
-    __syncthreads();
+    // ---- the rows that are written here: those of this workgroup's adapters and, in the first one, those without an adapter
+    uint64_t mine = 0;
+    int lead = -1;                                    // the first of these adapters
+    each_adapter(tile, [&](int cur, uint64_t rows) __attribute__((always_inline)) {
+        if (lead < 0) lead = cur;
+        mine |= rows;
+    });
+    const uint64_t idle = deal == 0 && a.outs != a.base ? tile.there & ~tile.with : 0;
+    if ((mine | idle) == 0) return;
 
+    const int first_column = (blockIdx.x * a.strips * 4 + wave) * 64;
+    const int end_column = min(a.S, (int)(blockIdx.x + 1) * a.strips * 256);
     const uint32_t row_bytes = 2u * (uint32_t)a.S;
-    const int c_end = min((int)(blockIdx.x + 1) * a.columns, a.S);
-    for (int c = blockIdx.x * a.columns + 64 * wave; c < c_end; c += 256) {
-        // tile j takes columns 4 n + j of the wave's 64
-        f32x4 sum[MT][4];
+    // rows of base and outs through buffers of the tile's rows: a row that is not to be read or written lies beyond
+    const int tile_bytes = (int)((uint32_t)min((int64_t)(16 * MT), a.rows - row0) * row_bytes);
+    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<h16*>(a.base) + row0 * a.S, 0, tile_bytes, AD_RSRC);
+    const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(a.outs + row0 * a.S, 0, tile_bytes, AD_RSRC);
+    auto offset = [&](int m, int r, uint64_t rows) __attribute__((always_inline)) {
+        const int row = 16 * m + 4 * q + r;
+        return ((uint32_t)row * row_bytes + 8u * n) | ((rows >> row) & 1 ? 0u : AD_BEYOND);
+    };
+    // ranks 32 ch + 8 q ... + 7 of columns 4 n ... 4 n + 3 of the strip at column c
+    auto load_up = [&](u32x2 (&w)[8], int adapter, int c, int ch) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<h16*>(a.up) + (int64_t)adapter * a.rank * a.S + c, 0, (int)((a.rank - 1) * row_bytes + 128u), AD_RSRC);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_raw_buffer_load_b64(rsrc, (uint32_t)(32 * ch + 8 * q + i) * row_bytes + 8u * n, 0, 0);
+    };
+    u32x2 ahead[PRE][8], base[MT][4];
+    uint32_t base_off[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) base_off[m][r] = offset(m, r, mine | idle);
+    // (beyond the last strip: the last column's again, not used)
+    auto ask_up = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int ch = 0; ch < PRE; ++ch) load_up(ahead[ch], max(lead, 0), min(c, a.S - 64), ch);       // (ranks that there are not read as 0)
+    };
+    auto ask_base = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        uint32_t mine = 0;                            // bit 4 m + r: row 16 m + 4 q + r is written here
-        int last = -1;
-        for (int index = 0;; ++index) {
-            const int cur = next_id<MT>(id, last);
-            if (cur == INT_MAX) break;
-            last = cur;
-            if (index % a.deal != deal) continue;
-            const __amdgpu_buffer_rsrc_t w_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<h16*>(a.up) + (int64_t)cur * a.rank * a.S + c, 0, (int)((a.rank - 1) * row_bytes + 128u), AD_RSRC);
+            for (int r = 0; r < 4; ++r) base[m][r] = __builtin_amdgcn_raw_buffer_load_b64(from, base_off[m][r], 2 * min(c, a.S - 64), 0);
+    };
+    ask_up(first_column);
+    ask_base(first_column);
+
+    // ---- h of these rows, 16, 32 or 64 lanes to a row
+    {
+        const int lanes = LONG || a.rank > 32 ? 64 : a.rank > 16 ? 32 : 16, per_wave = 64 / lanes;
+        const int sub = lane & (lanes - 1);
+#pragma unroll 1
+        for (int row = wave * per_wave + lane / lanes; row < 16 * MT; row += 4 * per_wave) {
+            const bool there = (mine >> row) & 1;
+            if (__builtin_amdgcn_ballot_w64(there) == 0) continue;
+            const int64_t at_row = row0 + row;
+            const int of = __shfl(tile.id, row);
+            const float scale = there ? a.scales[of] : 0.f;
+            float h[LONG ? 8 : 1], most = 0.f;
+#pragma unroll
+            for (int i = 0; i < (LONG ? 8 : 1); ++i) {
+                const int rank = 64 * i + sub;
+                float sum = 0.f;
+                if (there && rank < a.rank) {
+                    const float* const part = a.part + at_row * a.rank + rank;
+                    const int64_t next = a.rows * a.rank;
+                    int ks = 0;
+                    for (; ks + 4 <= a.ksplit; ks += 4)
+                        sum += (part[ks * next] + part[(ks + 1) * next]) + (part[(ks + 2) * next] + part[(ks + 3) * next]);
+                    for (; ks < a.ksplit; ++ks) sum += part[ks * next];
+                }
+                h[i] = sum * scale;
+                most = fmaxf(most, fabsf(h[i]));
+            }
+            most = dpp_fmax<0x140>(dpp_fmax<0x141>(dpp_fmax<0x4E>(dpp_fmax<0xB1>(most))));
+            if (lanes >= 32) most = fmaxf(most, __shfl_xor(most, 16));
+            if (lanes == 64) most = fmaxf(most, __shfl_xor(most, 32));
+            // most = f 2^e, f in [0.5, 1): times 2^(10 - e)
+            int e = 10;
+            if (most > 0.f && most < INFINITY) e = max(__builtin_amdgcn_frexp_expf(most), -100);
+            const float by = __builtin_ldexpf(1.f, 10 - e);
+#pragma unroll
+            for (int i = 0; i < (LONG ? 8 : 1); ++i) {
+                const float v = h[i] * by;
+                const h16 hi = (h16)v;
+                // (an infinity or NaN is in the high part alone)
+                const h16 lo = fabsf(v) < 65504.f ? (h16)(v - (float)hi) : (h16)0.f;
+                for (int rank = 64 * i + sub; rank < min(chunks * 32, 64 * i + 64); rank += lanes) {
+                    high[row * pitch + rank] = rank < 64 * i + lanes ? hi : (h16)0.f;
+                    low[row * pitch + rank] = rank < 64 * i + lanes ? lo : (h16)0.f;
+                }
+            }
+            if (sub == 0) unscale[row] = __builtin_ldexpf(1.f, e - 10);
+        }
+    }
+    __syncthreads();
+
+#pragma unroll 1
+    for (int c = first_column; c < end_column; c += 256) {
+        uint64_t left = tile.with & tile.dealt;
+        while (left) {
+            const int row = __builtin_ctzll(left), cur = __builtin_amdgcn_readlane(tile.id, row);
+            const uint64_t rows = __builtin_amdgcn_ballot_w64(tile.id == cur);
+            left &= ~rows;
+            if (__builtin_ctzll(rows) != row) continue;
             f32x4 acc[MT][4];
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            for (int ch = 0; ch < chunks; ++ch) {
-                // ranks 32 ch + 8 q ... + 7 of columns 4 n ... 4 n + 3, turned so that a register holds two ranks of a column
-                u32x2 w[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    w[i] = __builtin_amdgcn_raw_buffer_load_b64(w_rsrc, (uint32_t)(32 * ch + 8 * q + i) * row_bytes + 8u * n, 0, 0);
+            auto multiply = [&](const u32x2 (&w)[8], int ch) __attribute__((always_inline)) {
+                // turned so that a register holds two ranks of a column
                 h16x8 b[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -253,53 +290,72 @@ __global__ __launch_bounds__(256) void expand_kernel(AdapterArgs a) {
                         acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, b[j], acc[m][j], 0, 0, 0);
                     }
                 }
+            };
+            int ch = 0;
+            if (cur == lead) {
+#pragma unroll
+                for (int p = 0; p < PRE; ++p)
+                    if (p < chunks) multiply(ahead[p], p);
+                ch = PRE;
+                if (c + 256 < end_column) ask_up(c + 256);
             }
+            for (; ch < chunks; ++ch) {
+                u32x2 w[8];
+                load_up(w, cur, c, ch);
+                multiply(w, ch);
+            }
+            // register r of tile (m, j) is row 16 m + 4 q + r: this adapter's are done
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const f32x4 by = *reinterpret_cast<const f32x4*>(unscale + 16 * m + 4 * q);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const h16x4 v = bitcast<h16x4>(base[m][r]);
+                    h16x4 o;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[j] = (h16)((float)v[j] + acc[m][j][r] * by[r]);
+                    __builtin_amdgcn_raw_buffer_store_b64(bitcast<u32x2>(o), to, offset(m, r, rows), 2 * c, 0);
+                }
+            }
+        }
+        if (idle) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool of_cur = __shfl(id[m], 4 * q + r) == cur;
-                    mine |= of_cur ? 1u << (4 * m + r) : 0u;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sum[m][j][r] = of_cur ? acc[m][j][r] : sum[m][j][r];
-                }
+                for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b64(base[m][r], to, offset(m, r, idle), 2 * c, 0);
         }
-        // rows without an adapter are the first workgroup's
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const bool idle = __shfl(id[m], 4 * q + r) < 0;
-                const int row = 16 * m + 4 * q + r;
-                if (row0 + row < a.rows && (idle ? deal == 0 : (mine >> (4 * m + r)) & 1)) {
-                    const int64_t at = (row0 + row) * a.S + c + 4 * n;
-                    const h16x4 v = *reinterpret_cast<const h16x4*>(a.base + at);
-                    const float by = unscale[row];
-                    h16x4 o;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[j] = idle ? v[j] : (h16)((float)v[j] + sum[m][j][r] * by);
-                    *reinterpret_cast<h16x4*>(a.outs + at) = o;
-                }
-            }
+        if (c + 256 < end_column) ask_base(c + 256);
     }
 }
 
-struct AdapterPlan { int shrink_mt, nt, ksplit, units_per_split, expand_mt, columns, deal_shrink, deal_expand; };
+struct AdapterPlan { int mt, nt, ksplit, units_per_split, deal_shrink, deal_expand, strips; };
 
+// us, one side / the other, whole calls: the adapters of a tile dealt to 16 workgroups or not, 777 rows of 24 adapters 26 / 226; shares
+// of K of 8 units or of a thirtieth of it, the same rows 26 / 34; tiles of 16 or 32 rows for the second launch, 4096 rows of
+// prompts 97 / 86; workgroups that walk along the columns (1024 in all) or one for every 256 columns: 64 requests with an adapter of rank 64
+// each 49 / 53, 4096 rows of prompts 86 / 108.
 static AdapterPlan plan_adapters(const int4mm_adapter_shape& sh) {
     AdapterPlan p;
     const int64_t T = sh.rows, units = sh.in_size / 64;
+    auto tiles = [&](int mt) { return (T + 16 * mt - 1) / (16 * mt); };
+    // the most distinct adapters that a tile can hold, and the workgroups that its adapters are dealt to: until there are 2048
+    auto distinct = [&](int mt) { return std::min<int64_t>({sh.adapters, T, (16 * mt - 1) / std::min(sh.rows_per_id, T) + 2, 16 * mt}); };
+    auto deal = [&](int mt, int64_t workgroups) {
+        int d = 1;
+        while (d < distinct(mt) && d < 16 && d * workgroups < 2048) d *= 2;
+        return d;
+    };
     p.nt = sh.rank <= 16 ? 1 : sh.rank <= 32 ? 2 : 4;
-    p.shrink_mt = T <= 256 ? 1 : 2;
-    p.expand_mt = T <= 256 ? 1 : 4;
-    const bool many = T <= 256;
-    p.deal_shrink = many ? (int)std::min<int64_t>(16, std::min<int64_t>(T, sh.adapters)) : 1;
-    p.deal_expand = p.deal_shrink;
-    const int64_t tiles = (T + 16 * p.shrink_mt - 1) / (16 * p.shrink_mt) * ((sh.rank + 16 * p.nt - 1) / (16 * p.nt));
-    const int64_t want = std::max<int64_t>(1, 1024 / (many ? T : tiles));
-    p.units_per_split = (int)std::max<int64_t>(8, (units + want - 1) / want);
+    const int64_t rank_parts = (sh.rank + 16 * p.nt - 1) / (16 * p.nt);
+    p.mt = T <= 1024 ? 1 : 2;
+    p.deal_shrink = deal(p.mt, tiles(p.mt) * rank_parts);
+    // (a share is at least the two units that a wave takes at once, and there are at most 16 to add up)
+    const int64_t workgroups = tiles(p.mt) * rank_parts * p.deal_shrink;
+    p.units_per_split = (int)std::max<int64_t>({8, (units + 15) / 16, (units * workgroups + 8191) / 8192});
     p.ksplit = (int)((units + p.units_per_split - 1) / p.units_per_split);
-    p.columns = 256 * (T <= 256 ? 1 : 4);
+    const int64_t strips = (sh.out_size + 255) / 256;
+    p.deal_expand = deal(p.mt, tiles(p.mt) * strips);
+    p.strips = (int)std::max<int64_t>(1, tiles(p.mt) * p.deal_expand * strips / 1024);
     return p;
 }
 
@@ -354,14 +410,14 @@ int int4mm_low_rank_add(void* outs, const void* base, const void* x, const void*
     a.S = (int)sh->out_size;
     a.ksplit = p.ksplit;
     a.units_per_split = p.units_per_split;
-    a.columns = p.columns;
     hipStream_t st = (hipStream_t)stream;
     {
         a.deal = p.deal_shrink;
-        const dim3 grid(p.ksplit, (unsigned)((sh->rows + 16 * p.shrink_mt - 1) / (16 * p.shrink_mt)),
+        a.deal_rows = ~0ull / ((1ull << a.deal) - 1);
+        const dim3 grid(p.ksplit, (unsigned)((sh->rows + 16 * p.mt - 1) / (16 * p.mt)),
                         (unsigned)(p.deal_shrink * ((sh->rank + 16 * p.nt - 1) / (16 * p.nt))));
 #define SHRINK(MT, NT) hipLaunchKernelGGL((shrink_kernel<MT, NT>), grid, dim3(256), 0, st, a)
-        if (p.shrink_mt == 1) {
+        if (p.mt == 1) {
             if (p.nt == 1) SHRINK(1, 1); else if (p.nt == 2) SHRINK(1, 2); else SHRINK(1, 4);
         } else {
             if (p.nt == 1) SHRINK(2, 1); else if (p.nt == 2) SHRINK(2, 2); else SHRINK(2, 4);
@@ -370,11 +426,18 @@ int int4mm_low_rank_add(void* outs, const void* base, const void* x, const void*
         if (const int rc = check_launch("low_rank_add")) return rc;
     }
     a.deal = p.deal_expand;
-    const int height = 16 * p.expand_mt;
-    const dim3 grid((unsigned)((sh->out_size + p.columns - 1) / p.columns), (unsigned)((sh->rows + height - 1) / height), (unsigned)p.deal_expand);
+    a.deal_rows = ~0ull / ((1ull << a.deal) - 1);
+    a.strips = p.strips;
+    const int height = 16 * p.mt;
+    const dim3 grid((unsigned)((sh->out_size + 256 * p.strips - 1) / (256 * p.strips)), (unsigned)((sh->rows + height - 1) / height), (unsigned)p.deal_expand);
     const size_t lds = (size_t)height * (((sh->rank + 31) / 32 * 32 + 8) * 4 + 4);
-    if (p.expand_mt == 1) hipLaunchKernelGGL((expand_kernel<1>), grid, dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((expand_kernel<4>), grid, dim3(256), lds, st, a);
+#define EXPAND(MT)                                                                                    \
+    if (sh->rank <= 32) hipLaunchKernelGGL((expand_kernel<MT, false, 1>), grid, dim3(256), lds, st, a);     \
+    else if (sh->rank <= 64) hipLaunchKernelGGL((expand_kernel<MT, false, 2>), grid, dim3(256), lds, st, a); \
+    else hipLaunchKernelGGL((expand_kernel<MT, true, 2>), grid, dim3(256), lds, st, a)
+    if (p.mt == 1) { EXPAND(1); }
+    else { EXPAND(2); }
+#undef EXPAND
     return check_launch("low_rank_add");
 }
 
