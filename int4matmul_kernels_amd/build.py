@@ -22,7 +22,7 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "build")
 LIB = os.path.join(PKG, "libint4mm_hip.so")
 HIP_SOURCES = ["api.hip", "utils.hip", "matvec.hip", "matmul.hip", "skinny.hip", "wide.hip",
-               "route.hip", "experts.hip", "adapters.hip"]
+               "route.hip", "experts.hip", "experts_tiles.hip", "adapters.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 

@@ -12,26 +12,11 @@
 // in the loop: a lane loads 16 bytes of packed words, four neighbouring columns of the packed row that holds its 8 k, and each
 // word is after its decode the operand of one v_mfma_f32_16x16x32_f16 whose columns are every fourth of the strip; the states'
 // operands come straight from global memory, where the waves of all strips find them in the L2.  The partial sums meet in LDS.
-#include "decode.h"
+#include "experts.h"
 
 #include <algorithm>
 
 namespace i4 {
-
-struct ExpertsArgs {
-    const h16* x;                  // source rows
-    const uint32_t* matrix;
-    const uint32_t* mask;
-    const h16* scales;
-    const h16* zeros;
-    const int* offsets;            // [E + 1]: an expert's pairs among the ordered ones
-    const int* order;              // [P]: pair of each place
-    h16* h;                        // up: [P, F] by place
-    float* part;                   // down: [P, S] by place
-    int64_t matrix_stride, mask_stride, scale_stride;   // elements from an expert to the next
-    int experts, top_k, K, S;      // S: columns of the matrix (up: 2 F)
-    int group_units, strips;       // strips: of 64 columns
-};
 
 template <int BITS, bool SPARSE> struct RowsFmt;       // packed rows of a 32-row block, 16-byte loads of a lane per block
 template <> struct RowsFmt<4, false> { static constexpr int ROWS = 4, LOADS = 1; };
@@ -41,73 +26,91 @@ template <> struct RowsFmt<4, true> { static constexpr int ROWS = 2, LOADS = 3; 
 
 // ---- pairs in the order of their experts: workgroup e finds how many pairs belong to lower experts, and places its own.  Each
 // of the 16 waves takes a share of the pairs, twice: counting, then placing; no atomics, the order is that of the pairs.
+// A wave reads 256 pairs at a time, four neighbours a lane, and keeps the first 2048 of its share in registers: one trip to memory.
+struct __attribute__((packed, aligned(4))) FourIds { int v[4]; };
 __global__ __launch_bounds__(1024) void plan_kernel(const int* ids, int* offsets, int* order, int* place, int pairs, int experts) {
-    __shared__ int of_wave[16], lower;
+    constexpr int DEPTH = 8;
+    __shared__ int of_wave[16], lower_of_wave[16];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), e = blockIdx.x;
-    const int share = ((pairs + 15) / 16 + 63) & ~63, from = min(wave * share, pairs), to = min(from + share, pairs);
-    if (t == 0) lower = 0;
-    __syncthreads();
+    const int share = ((pairs + 15) / 16 + 255) & ~255, from = min(wave * share, pairs), to = min(from + share, pairs);
+    int kept[DEPTH][4];
+    auto load = [&](int (&v)[4], int at) __attribute__((always_inline)) {
+        const int p = at + 4 * lane;
+        if (p + 4 <= to) {
+            const FourIds f = *reinterpret_cast<const FourIds*>(ids + p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = f.v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = p + j < to ? ids[p + j] : -1;
+        }
+    };
     int mine = 0, below = 0;
-#pragma unroll 4
-    for (int i = from; i < to; i += 64) {
-        const int id = i + lane < to ? ids[i + lane] : -1;
-        mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(id == e));
-        below += __builtin_popcountll(__builtin_amdgcn_ballot_w64(id >= 0 && id < e));
+    auto count = [&](const int (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[j] == e));
+            below += __builtin_popcountll(__builtin_amdgcn_ballot_w64((uint32_t)v[j] < (uint32_t)e));
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (from + 256 * d < to) load(kept[d], from + 256 * d);
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (from + 256 * d < to) count(kept[d]);
+    for (int i = from + 256 * DEPTH; i < to; i += 256) {
+        int v[4];
+        load(v, i);
+        count(v);
     }
     if (lane == 0) {
         of_wave[wave] = mine;
-        atomicAdd(&lower, below);                     // (whole numbers: any order)
+        lower_of_wave[wave] = below;
     }
     __syncthreads();
-    int at = lower, all = 0;
+    int lower = 0, at = 0, all = 0;
+#pragma unroll
     for (int w = 0; w < 16; ++w) {
+        lower += lower_of_wave[w];
         at += w < wave ? of_wave[w] : 0;
         all += of_wave[w];
     }
+    at += lower;
     if (t == 0) {
         offsets[e] = lower;
         if (e == experts - 1) offsets[experts] = lower + all;
     }
-#pragma unroll 4
-    for (int i = from; i < to; i += 64) {
-        const int p = i + lane, id = p < to ? ids[p] : -1;
-        const uint64_t in = __builtin_amdgcn_ballot_w64(id == e);
-        if (id == e) {
-            const int where = at + __builtin_popcountll(in & ((1ull << lane) - 1));
-            order[where] = p;
-            place[p] = where;
-        } else if (e == 0 && p < to && (id < 0 || id >= experts)) {
-            place[p] = -1;
-        }
-        at += __builtin_popcountll(in);
-    }
-}
-
-// which expert's rows, and the first of them, is block `want` of blocks of `height` pairs each?  False: there are fewer blocks
-__device__ __forceinline__ bool find_block(const int* offsets, int experts, int height, int want, int lane, int& expert, int& first, int& count) {
-    for (int e0 = 0; e0 < experts; e0 += 64) {
-        const int e = e0 + lane;
-        const int a = offsets[min(e, experts)], b = offsets[min(e + 1, experts)];
-        const int blocks = (b - a + height - 1) / height;
-        int upto = blocks;                            // blocks of this lane's and the lower lanes' experts
+    const uint64_t before = (1ull << lane) - 1;
+    auto put = [&](const int (&v)[4], int i) __attribute__((always_inline)) {
+        uint64_t in[4];
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int o = __shfl_up(upto, d);
-            upto += lane >= d ? o : 0;
+        for (int j = 0; j < 4; ++j) in[j] = __builtin_amdgcn_ballot_w64(v[j] == e);
+        int where = at;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            where += __builtin_popcountll(in[j] & before);
+            at += __builtin_popcountll(in[j]);
         }
-        const uint64_t beyond = __builtin_amdgcn_ballot_w64(upto > want);
-        if (beyond) {
-            const int l = __builtin_ctzll(beyond);
-            expert = e0 + l;
-            const int nth = want - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(blocks, l));
-            const int from = __builtin_amdgcn_readlane(a, l), to = __builtin_amdgcn_readlane(b, l);
-            first = from + nth * height;
-            count = min(height, to - first);
-            return true;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int p = i + 4 * lane + j;
+            if (v[j] == e) {
+                order[where] = p;
+                place[p] = where++;
+            } else if (e == 0 && p < to && (uint32_t)v[j] >= (uint32_t)experts) {
+                place[p] = -1;
+            }
         }
-        want -= __builtin_amdgcn_readlane(upto, 63);
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (from + 256 * d < to) put(kept[d], from + 256 * d);
+    for (int i = from + 256 * DEPTH; i < to; i += 256) {
+        int v[4];
+        load(v, i);
+        put(v, i);
     }
-    return false;
 }
 
 // ---- a product of up to 16 MT pairs of one expert with 64 columns.  UP: 32 columns of the gate and the same 32 of the other
@@ -120,8 +123,9 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(ExpertsArgs a) {
     __shared__ __attribute__((aligned(16))) uint32_t lut[SPARSE ? SPARSE_LUT_WORDS : 4];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, q = lane >> 4;
-    int expert, first, count;
-    if (!find_block(a.offsets, a.experts, HEIGHT, blockIdx.x / a.strips, lane, expert, first, count)) return;
+    Block block;
+    if (find_block(a.offsets, a.experts, HEIGHT, blockIdx.x / a.strips, lane, block) >= 0) return;
+    const int expert = block.expert, first = block.first, count = block.count;
     const int strip = blockIdx.x % a.strips;
     if constexpr (SPARSE) {
         for (int e = t; e < 256; e += 64 * WAVES) {
@@ -240,7 +244,7 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(ExpertsArgs a) {
             const f32x4 gate = total(row, c), up = total(row, c + 32);
             h16x4 o;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = (h16)(gate[j] / (1.f + __expf(-gate[j])) * up[j]);
+            for (int j = 0; j < 4; ++j) o[j] = (h16)silu_times(gate[j], up[j]);
             *reinterpret_cast<h16x4*>(a.h + (int64_t)(first + row) * half + 32 * strip + c) = o;
         } else {
             *reinterpret_cast<f32x4*>(a.part + (int64_t)(first + row) * a.S + 64 * strip + c) = total(row, c);
@@ -248,17 +252,29 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(ExpertsArgs a) {
     }
 }
 
-// outs[t, :] = sum over j of weights[t, j] part[place[t, j], :]; a thread takes four columns
-__global__ __launch_bounds__(256) void combine_kernel(h16* outs, const float* part, const float* weights, const int* place, int top_k, int S, int parts) {
+// outs[t, :] = sum over j of weights[t, j] part[place[t, j], :]; a thread takes four columns (fp32) or eight (fp16)
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(h16* outs, const T* part, const float* weights, const int* place, int top_k, int S, int parts) {
+    constexpr int N = 16 / sizeof(T);
+    typedef T Vec __attribute__((ext_vector_type(N)));
+    typedef h16 Out __attribute__((ext_vector_type(N)));
     const int64_t t = blockIdx.x / parts;
-    const int c = ((int)(blockIdx.x % parts) * 256 + threadIdx.x) * 4;
+    const int c = ((int)(blockIdx.x % parts) * 256 + threadIdx.x) * N;
     if (c >= S) return;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    float sum[N] = {};
+#pragma unroll 4
     for (int j = 0; j < top_k; ++j) {
         const int p = place[t * top_k + j];
-        if (p >= 0) sum += weights[t * top_k + j] * *reinterpret_cast<const f32x4*>(part + (int64_t)p * S + c);
+        if (p < 0) continue;
+        const float w = weights[t * top_k + j];
+        const Vec v = *reinterpret_cast<const Vec*>(part + (int64_t)p * S + c);
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] += w * (float)v[i];
     }
-    *reinterpret_cast<h16x4*>(outs + t * S + c) = h16x4{(h16)sum[0], (h16)sum[1], (h16)sum[2], (h16)sum[3]};
+    Out o;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = (h16)sum[i];
+    *reinterpret_cast<Out*>(outs + t * S + c) = o;
 }
 
 template <int BITS, bool SPARSE, bool UP>
@@ -357,6 +373,8 @@ int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weig
     // pairs per expert, if all are asked alike
     const int64_t mean = pairs / E;
     const int mt = mean <= 8 ? 1 : mean <= 24 ? 2 : 4;
+    const bool tiles = mean >= 64;
+    const int tm = mean < 96 ? 2 : mean < 256 ? 4 : 8;
     auto rows_of = [&](int64_t k) { return sparse ? k / 16 : k * bits / 32; };
     a.x = static_cast<const h16*>(x);
     a.matrix = static_cast<const uint32_t*>(up_matrix);
@@ -368,7 +386,9 @@ int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weig
     a.matrix_stride = rows_of(K) * 2 * F;
     a.mask_stride = K / 32 * 2 * F;
     a.scale_stride = sh->up_groups * 2 * F;
-    rows_product<true>(bits, a, mt, pairs, st);
+    a.x_bytes = (uint32_t)(sh->tokens * K * 2);
+    if (tiles) launch_experts_tiles(bits, a, tm, pairs, true, st);
+    else rows_product<true>(bits, a, mt, pairs, st);
     if (const int rc = check_launch("experts_forward")) return rc;
     a.x = a.h;
     a.matrix = static_cast<const uint32_t*>(down_matrix);
@@ -380,11 +400,21 @@ int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weig
     a.matrix_stride = rows_of(F) * K;
     a.mask_stride = F / 32 * K;
     a.scale_stride = sh->down_groups * K;
-    rows_product<false>(bits, a, mt, pairs, st);
+    if (tiles) {
+        a.h = reinterpret_cast<h16*>(ws + parts.part);
+        launch_experts_tiles(bits, a, tm, pairs, false, st);
+    } else {
+        rows_product<false>(bits, a, mt, pairs, st);
+    }
     if (const int rc = check_launch("experts_forward")) return rc;
-    const int columns = (int)((K / 4 + 255) / 256);
-    hipLaunchKernelGGL(combine_kernel, dim3((unsigned)(sh->tokens * columns)), dim3(256), 0, st, static_cast<h16*>(outs), a.part, static_cast<const float*>(weights), place,
+    const int columns = (int)((K + (tiles ? 2047 : 1023)) / (tiles ? 2048 : 1024));
+    const dim3 grid((unsigned)(sh->tokens * columns));
+    if (tiles)
+        hipLaunchKernelGGL(combine_kernel<h16>, grid, dim3(256), 0, st, static_cast<h16*>(outs), a.h, static_cast<const float*>(weights), place,
                            a.top_k, (int)K, columns);
+    else
+        hipLaunchKernelGGL(combine_kernel<float>, grid, dim3(256), 0, st, static_cast<h16*>(outs), a.part, static_cast<const float*>(weights),
+                           place, a.top_k, (int)K, columns);
     return check_launch("experts_forward");
 }
 
