@@ -12,6 +12,7 @@ namespace i4 {
 // The coefficients of a column's group: {s, s}, {z, z} or what the decode makes of them.
 // Linear mode: the reference's own two roundings, fp16(q - z), fp16(. * s).
 struct LinearCoef {
+    static constexpr bool EITHER = false;
     h16x2 s, z;
     __device__ __forceinline__ void set(h16x2 s2, h16x2 z2) { s = s2; z = z2; }
     __device__ __forceinline__ uint32_t weight(h16x2 q) const { return as_u32((q - z) * s); }
@@ -21,6 +22,7 @@ struct LinearCoef {
 // linear:   P = q, N = -z, B = s, C = -0:  fp16(q - z), then fp16(. * s) -- adding -0 changes nothing
 // exponent: P = +-2^e, N = -0, B = -s, C = z:  the reference's single-rounded fma (matmul.cuh:127-136)
 struct TwoModeCoef {
+    static constexpr bool EITHER = true;
     uint32_t m;                                  // all ones in exponent mode (bit picks: a selection came out as a branch)
     h16x2 N, B, C;
     float scale;                                 // of the 8-bit floats: 2^9 for q, 1 for +-2^e
@@ -60,11 +62,49 @@ struct Int3Coef : TwoModeCoef {
 template <int BITS, bool TWO_MODES>
 using Coef = std::conditional_t<BITS == 2, Int2Coef, std::conditional_t<BITS == 3, Int3Coef, std::conditional_t<TWO_MODES, TwoModeCoef, LinearCoef>>>;
 
+// What the codes stand for alone, exact in fp16: q or, in a column in exponent mode, +-2^e.  Scale and zero are left to the sums:
+//     sum x w = A sum x value + B sum x,   (A, B) = (s, -s z), in exponent mode (-s, z)
+template <int BITS>
+struct CodeValues {
+    static constexpr bool EITHER = false;
+    static constexpr uint32_t T0 = BITS == 2 ? 0x3C000000u : 0x42403C00u, T1 = BITS == 2 ? 0x42004000u : 0x47464544u;
+    __device__ __forceinline__ void set(h16x2, h16x2) {}
+    __device__ __forceinline__ uint32_t weight(h16x2 value) const { return as_u32(value); }
+};
+template <int BITS>
+struct EitherValues : TwoModeCoef {
+    uint32_t T0, T1;
+    __device__ __forceinline__ void set(h16x2 s2, h16x2 z2) {
+        TwoModeCoef::set(s2, z2);
+        T0 = BITS == 2 ? pick(0x40003C00u, 0x3C000000u) : pick(0x4844403Cu, 0x42403C00u);
+        T1 = BITS == 2 ? pick(0xC000BC00u, 0x42004000u) : pick(0xC8C4C0BCu, 0x47464544u);
+    }
+    __device__ __forceinline__ uint32_t weight(h16x2 value) const { return as_u32(value); }
+};
+// 16:32: a dropped row must not meet the zero either, so that is subtracted here, the one rounding; a column in exponent mode is
+// complete
+//     sum x w = A sum x value,   A = s, in exponent mode 1
+struct KeptValues {
+    static constexpr bool EITHER = false;
+    h16x2 z;
+    __device__ __forceinline__ void set(h16x2, h16x2 z2) { z = z2; }
+    __device__ __forceinline__ uint32_t weight(h16x2 q) const { return as_u32(q - z); }
+};
+struct EitherKeptValues : TwoModeCoef {
+    __device__ __forceinline__ void set(h16x2 s2, h16x2 z2) {
+        TwoModeCoef::set(s2, z2);
+        B = as_h2(pick(as_u32(B), 0x3C003C00u));
+    }
+};
+template <int BITS, bool SPARSE, bool EITHER>
+using Values = std::conditional_t<SPARSE, std::conditional_t<EITHER, EitherKeptValues, KeptValues>,
+                                  std::conditional_t<EITHER, EitherValues<BITS>, CodeValues<BITS>>>;
+
 // four codes of a word as bytes -> eight weights: a byte q < 16 is the 8-bit float q 2^-9
 template <class C>
 __device__ __forceinline__ h16x8 weights_of_bytes(uint32_t b03, uint32_t b47, const C& c) {
     float scale = 512.f;
-    if constexpr (std::is_same_v<C, TwoModeCoef>) {
+    if constexpr (C::EITHER) {
         b03 = c.powers(b03);
         b47 = c.powers(b47);
         scale = c.scale;

@@ -18,7 +18,8 @@ struct ExpertsArgs {
     int64_t matrix_stride, mask_stride, scale_stride;   // elements from an expert to the next
     int experts, top_k, K, S;      // S: columns of the matrix (up: 2 F)
     int group_units, strips;       // strips: of columns
-    uint32_t x_bytes;              // tiles: of all source rows
+    uint32_t group_magic;
+    uint32_t x_bytes;              // up: of all source rows
 };
 
 // Blocks of up to `height` pairs of one expert, in the order of the experts.  `expert`, `first` and `count` of block `want`;

@@ -1,17 +1,24 @@
 // The experts' gated feed-forward on packed weights: of tokens x [T, K] with the experts ids [T, k] and their weights [T, k]
 //     h[t, j, :] = silu(x[t] up_e[:, :F]) * (x[t] up_e[:, F:]),   outs[t, :] = fp16( sum_j weights[t, j] * (h[t, j] down_e) ),
-// e = ids[t, j]; a pair whose id is outside 0 ... E - 1 has no expert and adds nothing.  Every weight is dequantised as the
-// products of the linear layers do it, fp16(fp16(q - z) s) or the exponent mode's fma, sums are fp32, h is rounded to fp16 (it
-// is an operand of the matrix instructions), and so is the result.
+// e = ids[t, j]; a pair whose id is outside 0 ... E - 1 has no expert and adds nothing.  Sums are fp32; h is rounded to fp16 (it is
+// an operand of the matrix instructions), and so is the result.
 //
 //   plan_kernel     pairs in the order of their experts, stable: where each expert's begin, the pairs, each pair's place
-//   rows_kernel     a product of the pairs of one expert, up to 16 MT at a time, with a strip of 64 columns
+//   rows_kernel     a product of the pairs of one expert, up to 16 MT at a time, with a strip of 64 columns (many pairs an expert:
+//                   experts_tiles.hip)
 //   combine_kernel  the weighted sum of a token's k results, fp32
 //
-// rows_kernel is bound by reading the packed weights.  The waves of a workgroup share K out, so nothing is shared through LDS
-// in the loop: a lane loads 16 bytes of packed words, four neighbouring columns of the packed row that holds its 8 k, and each
-// word is after its decode the operand of one v_mfma_f32_16x16x32_f16 whose columns are every fourth of the strip; the states'
-// operands come straight from global memory, where the waves of all strips find them in the L2.  The partial sums meet in LDS.
+// rows_kernel is bound by reading the packed weights and by the instructions that decode them.  The waves of a workgroup share K out,
+// so nothing is shared through LDS in the loop: a lane loads 16 bytes of packed words, four neighbouring columns of the packed row
+// that holds its 8 k, and each word is after its decode the operand of one v_mfma_f32_16x16x32_f16 whose columns are every fourth
+// of the strip.  Blocks of up to 32 pairs multiply what the codes stand for, exact in fp16, and apply scale and zero once per group
+// to the sums (sum x w = s (sum x q - z sum x), the sum of x from a product with ones), which takes 7 instructions a word where
+// rounded weights take 17 and is nearer to the exact product; 64 pairs have no registers for it and round their weights as the tile
+// kernels do.  The partial sums of the waves meet in LDS.
+//
+// Measured (64 tokens, two of eight experts of 4096 x 11008, int4, us a call): weights rounded, addresses computed, one lane for 16
+// bytes of every row of states 198; exact codes, buffer loads, two units in flight in the order that the waits go by 178; states
+// read row by row and turned in LDS 160.
 #include "experts.h"
 
 #include <algorithm>
@@ -115,11 +122,14 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int* ids, int* offsets
 
 // ---- a product of up to 16 MT pairs of one expert with 64 columns.  UP: 32 columns of the gate and the same 32 of the other
 // half; the source row of a pair is its token's, the result h.  Else: 64 columns, source and result by place.
-template <int BITS, bool SPARSE, int MT, int WAVES, bool UP>
-__global__ __launch_bounds__(64 * WAVES) void rows_kernel(ExpertsArgs a) {
+template <int BITS, bool SPARSE, int MT, int WAVES, int DEPTH, bool UP>
+__global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(ExpertsArgs a) {
     using F = RowsFmt<BITS, SPARSE>;
-    constexpr int HEIGHT = 16 * MT;
+    constexpr int HEIGHT = 16 * MT, RSRC = 0x00020000;
+    // sums of what the codes stand for, scale and zero once per group; tall blocks have no registers for it and round their weights
+    constexpr bool VALUES = MT <= 2, SUM_X = VALUES && !SPARSE;
     __shared__ __attribute__((aligned(16))) float red[WAVES * HEIGHT * 64];
+    __shared__ __attribute__((aligned(16))) char staged[WAVES * HEIGHT * 128];
     __shared__ __attribute__((aligned(16))) uint32_t lut[SPARSE ? SPARSE_LUT_WORDS : 4];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, q = lane >> 4;
@@ -139,97 +149,172 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(ExpertsArgs a) {
     const int half = a.S / 2;
     // lane n's four columns of the strip
     const int col = UP ? (n < 8 ? 0 : half - 32) + 32 * strip + 4 * n : 64 * strip + 4 * n;
-    const h16* xrow[MT];
+    // every load is a buffer, an offset of the lane that does not change and a uniform one that moves with k
+    const int units = a.K / 64, groups = (units + a.group_units - 1) / a.group_units;
+    const uint32_t row_bytes = 4u * (uint32_t)a.S;
+    auto buffer = [](const void* p, uint32_t bytes) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, RSRC); };
+    const __amdgpu_buffer_rsrc_t w_rsrc = buffer(a.matrix + expert * a.matrix_stride, 2 * units * F::ROWS * row_bytes);
+    const __amdgpu_buffer_rsrc_t m_rsrc = buffer(SPARSE ? a.mask + expert * a.mask_stride : a.matrix, 2 * units * row_bytes);
+    const __amdgpu_buffer_rsrc_t s_rsrc = buffer(a.scales + expert * a.scale_stride, groups * (row_bytes / 2));
+    const __amdgpu_buffer_rsrc_t z_rsrc = buffer(a.zeros + expert * a.scale_stride, groups * (row_bytes / 2));
+    const __amdgpu_buffer_rsrc_t x_rsrc = UP ? buffer(a.x, a.x_bytes) : buffer(a.x + (int64_t)first * a.K, 2u * (uint32_t)count * a.K);
+    // states: eight lanes read the 128 bytes of a row (one lane for 16 bytes of every row, as the operands want them, are 64 accesses of
+    // the L1 a load, four times as many), and the wave turns them in LDS of its own: chunk c of row r stands at c ^ (r % 8)
+    uint32_t x_off[2 * MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int at = first + min(16 * m + n, count - 1);              // (rows beyond the last repeat it and are not written)
-        xrow[m] = a.x + (int64_t)(UP ? a.order[at] / a.top_k : at) * a.K + 8 * q;
+    for (int i = 0; i < 2 * MT; ++i) {
+        const int at = min(8 * i + (lane >> 3), count - 1);             // (rows beyond the last repeat it and are not written)
+        x_off[i] = 2u * ((uint32_t)(UP ? a.order[first + at] / a.top_k : at) * a.K + 8 * (lane & 7));
     }
-    const uint32_t* const matrix = a.matrix + expert * a.matrix_stride;
-    const uint32_t* const mask = SPARSE ? a.mask + expert * a.mask_stride : nullptr;
-    const h16* const scales = a.scales + expert * a.scale_stride + col;
-    const h16* const zeros = a.zeros + expert * a.scale_stride + col;
-
-    f32x4 acc[MT][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // (written and read as the same type: without a barrier between, the compiler has to see that they are the same memory)
+    char* const stage = staged + wave * (HEIGHT * 128);
+    char* const stage_to = stage + (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16;
+    const uint32_t row0 = BITS == 4 && !SPARSE ? q : BITS == 2 ? q >> 1 : BITS == 3 ? (q > 0 ? q - 1 : 0) : 0;
+    const uint32_t w_off = 4u * col + row0 * row_bytes, w_off2 = 4u * col + (SPARSE ? 1 : min(row0 + 1, 2u)) * row_bytes;
 
     struct Unit {                                     // 64 k
         u32x4 w[2][F::LOADS];
-        u32x4 x[2][MT];
         u32x2 s, z;
     };
-    const uint32_t row0 = BITS == 4 && !SPARSE ? q : BITS == 2 ? q >> 1 : BITS == 3 ? (q > 0 ? q - 1 : 0) : 0;
     auto load = [&](Unit& u, int unit) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const uint32_t* const blk = matrix + (int64_t)(2 * unit + b) * F::ROWS * a.S + col;
-            u.w[b][0] = *reinterpret_cast<const u32x4*>(blk + (uint32_t)(row0 * a.S));
-            if constexpr (BITS == 3) u.w[b][1] = *reinterpret_cast<const u32x4*>(blk + (uint32_t)(min((int)row0 + 1, 2) * a.S));
-            if constexpr (SPARSE) {
-                u.w[b][1] = *reinterpret_cast<const u32x4*>(blk + a.S);
-                u.w[b][2] = *reinterpret_cast<const u32x4*>(mask + (int64_t)(2 * unit + b) * a.S + col);
-            }
-#pragma unroll
-            for (int m = 0; m < MT; ++m) u.x[b][m] = *reinterpret_cast<const u32x4*>(xrow[m] + 64 * unit + 32 * b);
+            const uint32_t blk = (uint32_t)(2 * unit + b) * row_bytes;
+            u.w[b][0] = __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, w_off, blk * F::ROWS, 0);
+            if constexpr (F::LOADS > 1) u.w[b][1] = __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, w_off2, blk * F::ROWS, 0);
+            if constexpr (SPARSE) u.w[b][2] = __builtin_amdgcn_raw_buffer_load_b128(m_rsrc, 4u * col, blk, 0);
         }
-        const int64_t g = (int64_t)(unit / a.group_units) * a.S;
-        u.s = *reinterpret_cast<const u32x2*>(scales + g);
-        u.z = *reinterpret_cast<const u32x2*>(zeros + g);
+        const uint32_t g = (uint32_t)magic_div(unit, a.group_units, a.group_magic) * (row_bytes / 2);
+        u.s = __builtin_amdgcn_raw_buffer_load_b64(s_rsrc, 2u * col, g, 0);
+        u.z = __builtin_amdgcn_raw_buffer_load_b64(z_rsrc, 2u * col, g, 0);
     };
-    auto multiply = [&](auto mode, const Unit& u) __attribute__((always_inline)) {
-        Coef<BITS, decltype(mode)::value> co[4];
+
+    f32x4 acc[MT][4], acc_x[MT], sum[VALUES ? MT : 1][4];
+    auto clear = [&](auto& v) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t sel = (j & 1) ? 0x03020302u : 0x01000100u;
-            co[j].set(as_h2(__builtin_amdgcn_perm(u.s[j >> 1], u.s[j >> 1], sel)), as_h2(__builtin_amdgcn_perm(u.z[j >> 1], u.z[j >> 1], sel)));
-        }
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    auto clear_group = [&]() __attribute__((always_inline)) {
+        clear(acc);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc_x[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    clear_group();
+    if constexpr (VALUES) clear(sum);
+    const h16x8 ones = bitcast<h16x8>(u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
+    auto multiply = [&](auto mode, const Unit& u) __attribute__((always_inline)) {
+        constexpr bool either = decltype(mode)::value;
+        h16x8 x[2][MT];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int m = 0; m < MT; ++m)
+                x[b][m] = bitcast<h16x8>(*reinterpret_cast<const u32x4*>(stage + (16 * m + n) * 128 + (((4 * b + q) ^ n) & 7) * 16));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            std::conditional_t<VALUES, Values<BITS, SPARSE, either>, Coef<BITS, either>> co;
+            const uint32_t sel = (j & 1) ? 0x03020302u : 0x01000100u;
+            co.set(as_h2(__builtin_amdgcn_perm(u.s[j >> 1], u.s[j >> 1], sel)), as_h2(__builtin_amdgcn_perm(u.z[j >> 1], u.z[j >> 1], sel)));
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
                 h16x8 w;
                 if constexpr (SPARSE) {
                     const uint32_t m = u.w[b][2][j], m8 = (m >> (8 * q)) & 0xFFu;
                     const uint32_t skip = __builtin_popcount(m & ((1u << (8 * q)) - 1u));
-                    const uint64_t st = ((uint64_t)u.w[b][1][j] << 32) | u.w[b][0][j];
-                    w = dequant_chunk_sparse((uint32_t)((st >> (2 * skip)) >> (2 * skip)), m8, lut, co[j]);
+                    // the codes from the skip-th on.  (Not a shift of 64 bits: with its amount in the last vector register that a
+                    // kernel has, this GPU shifts by something else now and then, and the compiler does not keep from it.)
+                    const uint32_t lo = u.w[b][0][j], hi = u.w[b][1][j];
+                    w = dequant_chunk_sparse(__builtin_amdgcn_alignbit(skip < 8 ? hi : 0u, skip < 8 ? lo : hi, 4 * skip), m8, lut, co);
                 } else if constexpr (BITS == 4) {
-                    w = dequant_chunk<4>(u.w[b][0][j], co[j]);
+                    w = dequant_chunk<4>(u.w[b][0][j], co);
                 } else if constexpr (BITS == 2) {
-                    w = dequant_chunk<2>(u.w[b][0][j] >> (16 * (q & 1)), co[j]);
+                    w = dequant_chunk<2>(u.w[b][0][j] >> (16 * (q & 1)), co);
                 } else {
                     // bits 24 q ... 24 q + 23 of the 96
                     const uint32_t lo = u.w[b][0][j], hi = u.w[b][1][j];
-                    w = dequant_chunk<3>(q == 0 ? lo : q == 1 ? __builtin_amdgcn_alignbit(hi, lo, 24) : q == 2 ? __builtin_amdgcn_alignbit(hi, lo, 16) : hi >> 8, co[j]);
+                    w = dequant_chunk<3>(__builtin_amdgcn_alignbit(q == 3 ? 0u : hi, q == 3 ? hi : lo, (32 - 8 * q) & 31), co);
                 }
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
-                    acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<h16x8>(u.x[b][m]), w, acc[m][j], 0, 0, 0);
+                for (int m = 0; m < MT; ++m) acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[b][m], w, acc[m][j], 0, 0, 0);
             }
+        }
+        if constexpr (SUM_X) {
+            // (every column of this product is the rows' sums: a lane has those of the rows that it has results of)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc_x[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[b][m], ones, acc_x[m], 0, 0, 0);
+        }
     };
-    const int units = a.K / 64, u0 = units * wave / WAVES, u1 = units * (wave + 1) / WAVES;
-    auto take = [&](const Unit& now) __attribute__((always_inline)) {
-        // a negative or NaN scale anywhere in the wave: the decode that serves either mode
-        if (BITS == 4 && __builtin_amdgcn_ballot_w64(((now.s[0] | now.s[1]) & 0x80008000u) != 0) != 0) multiply(std::bool_constant<BITS == 4>{}, now);
-        else multiply(std::false_type{}, now);
+    // the end of a group, or of the wave's part of one
+    auto fold = [&](const Unit& u) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float s = (float)as_h2(u.s[j >> 1])[j & 1], z = (float)as_h2(u.z[j >> 1])[j & 1];
+            const bool linear = s >= 0.f;
+            const float A = SPARSE ? (linear ? s : 1.f) : linear ? s : -s, B = linear ? -s * z : z;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if constexpr (SUM_X) sum[m][j][r] = fmaf(B, acc_x[m][r], sum[m][j][r]);
+                    sum[m][j][r] = fmaf(A, acc[m][j][r], sum[m][j][r]);
+                }
+        }
+        clear_group();
     };
-    Unit ua, ub;
-    if (u0 < u1) load(ua, u0);
-    for (int i = u0; i < u1; i += 2) {
-        if (i + 1 < u1) load(ub, i + 1);
-        take(ua);
-        if (i + 2 < u1) load(ua, i + 2);
-        if (i + 1 < u1) take(ub);
+    const int u0 = units * wave / WAVES, u1 = units * (wave + 1) / WAVES;
+    // DEPTH units in flight; what would be beyond the last is the last again, from the L1 (a load under a condition would make
+    // the compiler wait for more than it needs)
+    if (u0 < u1) {
+        int left = a.group_units - (u0 - magic_div(u0, a.group_units, a.group_magic) * a.group_units);
+        Unit ring[DEPTH];
+        u32x4 x[2 * MT];                              // the next unit's: they come from the L2
+        auto load_x = [&](int unit) __attribute__((always_inline)) {
+#pragma unroll
+            for (int c = 0; c < 2 * MT; ++c) x[c] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, x_off[c], 128u * unit, 0);
+        };
+        load_x(u0);
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            load(ring[d], min(u0 + d, u1 - 1));
+            __builtin_amdgcn_sched_barrier(0);        // (in this order, which the waits in the loop go by)
+        }
+#pragma unroll 1
+        for (int i = u0; i < u1; i += DEPTH) {
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                const Unit& now = ring[d];
+#pragma unroll
+                for (int c = 0; c < 2 * MT; ++c) *reinterpret_cast<u32x4*>(stage_to + c * 1024) = x[c];
+                load_x(min(i + d + 1, u1 - 1));
+                __builtin_amdgcn_sched_barrier(0);
+                if (i + d < u1) {
+                    // a negative or NaN scale anywhere in the wave: the decode that serves either mode
+                    const bool negative = __builtin_amdgcn_ballot_w64(((now.s[0] | now.s[1]) & 0x80008000u) != 0) != 0;
+                    if ((VALUES || BITS == 4) && negative) multiply(std::bool_constant<VALUES || BITS == 4>{}, now);
+                    else multiply(std::false_type{}, now);
+                    if constexpr (VALUES) {
+                        if (--left == 0 || i + d == u1 - 1) {
+                            fold(now);
+                            left = a.group_units;
+                        }
+                    }
+                }
+                load(ring[d], min(i + d + DEPTH, u1 - 1));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
     }
+    auto& result = [&]() -> auto& { if constexpr (VALUES) return sum; else return acc; }();
     // register r of tile (m, j): row 16 m + 4 q + r, column 4 n + j of the strip
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            *reinterpret_cast<f32x4*>(red + (wave * HEIGHT + 16 * m + 4 * q + r) * 64 + 4 * n) = f32x4{acc[m][0][r], acc[m][1][r], acc[m][2][r], acc[m][3][r]};
+            *reinterpret_cast<f32x4*>(red + (wave * HEIGHT + 16 * m + 4 * q + r) * 64 + 4 * n) = f32x4{result[m][0][r], result[m][1][r], result[m][2][r], result[m][3][r]};
     __syncthreads();
     auto total = [&](int row, int c) __attribute__((always_inline)) {
         f32x4 s = *reinterpret_cast<const f32x4*>(red + row * 64 + c);
@@ -282,9 +367,9 @@ static void launch_rows(ExpertsArgs a, int mt, int64_t pairs, hipStream_t st) {
     a.strips = a.S / 64;
     const int64_t height = 16 * mt, blocks = std::min<int64_t>(pairs, a.experts + pairs / height);
     const dim3 grid((unsigned)(blocks * a.strips));
-    if (mt == 1) hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 1, 8, UP>), grid, dim3(512), 0, st, a);
-    else if (mt == 2) hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 2, 4, UP>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 4, 4, UP>), grid, dim3(256), 0, st, a);
+    if (mt == 1) hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 1, 8, 2, UP>), grid, dim3(512), 0, st, a);
+    else if (mt == 2) hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 2, 4, 2, UP>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 4, 4, 2, UP>), grid, dim3(256), 0, st, a);
 }
 
 template <bool UP>
@@ -304,8 +389,8 @@ static int check_experts(int bits, const int4mm_experts_shape* sh, bool sparse) 
     if (g == 0 || (g > 0 && g % 64 != 0)) return INT4MM_ERR_GROUP;
     const int64_t up_groups = g < 0 ? 1 : (K + g - 1) / g, down_groups = g < 0 ? 1 : (F + g - 1) / g;
     if (sh->up_groups != up_groups || sh->down_groups != down_groups) return INT4MM_ERR_SHAPE;
-    // (a row of a block is addressed with 32 bits from the block's first, and a grid has so many rows)
-    if (K > limit / 64 || F > limit / 64 || K * F >= limit * 16) return INT4MM_ERR_SHAPE;
+    // (a matrix, and the rows of a block, are addressed with 31 bits)
+    if (K >= limit / 128 || F >= limit / 128 || K * F >= limit) return INT4MM_ERR_SHAPE;
     // (grids of one dimension: a workgroup per 16 pairs or expert and 64 columns)
     if (sh->top_k > 1024 || sh->tokens > limit || (sh->tokens * sh->top_k / 16 + sh->experts) * (std::max(K, 2 * F) / 64) >= limit ||
         sh->tokens * sh->top_k >= limit / 2)
@@ -366,7 +451,8 @@ int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weig
     a.part = reinterpret_cast<float*>(ws + parts.part);
     a.experts = E;
     a.top_k = (int)sh->top_k;
-    a.group_units = (int)(sh->group_size < 0 ? ONE_GROUP / 64 : sh->group_size / 64);
+    a.group_units = (int)(sh->group_size < 0 ? std::max(K, F) / 64 : std::min(sh->group_size, std::max(K, F) + 63) / 64);
+    a.group_magic = div_magic((uint32_t)a.group_units);
     hipLaunchKernelGGL(plan_kernel, dim3(E), dim3(1024), 0, st, static_cast<const int*>(ids), const_cast<int*>(a.offsets),
                            const_cast<int*>(a.order), place, (int)pairs, E);
     if (const int rc = check_launch("experts_forward")) return rc;
