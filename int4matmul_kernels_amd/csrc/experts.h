@@ -15,6 +15,10 @@ struct ExpertsArgs {
     const int* order;              // [P]: pair of each place
     h16* h;                        // up: [P, F] by place; tiles of the second product: [P, S]
     float* part;                   // down: [P, S] by place
+    const int* ids;
+    const float* weights;
+    h16* outs;
+    int* arrivals;                 // pairs by themselves: [tokens, strips] workgroups that have stored their sums
     int64_t matrix_stride, mask_stride, scale_stride;   // elements from an expert to the next
     int experts, top_k, K, S;      // S: columns of the matrix (up: 2 F)
     int group_units, strips;       // strips: of columns

@@ -120,12 +120,60 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int* ids, int* offsets
     }
 }
 
+// The operand of a lane, 8 k of one column, from the words that it has loaded of a 32-row block: `lo` its packed word (int3: and the
+// next, 16:32: and the block's second and its mask)
+template <int BITS, bool SPARSE, class C>
+__device__ __forceinline__ h16x8 operand_of(uint32_t lo, uint32_t hi, uint32_t mask, int q, const uint32_t* lut, const C& co) {
+    if constexpr (SPARSE) {
+        const uint32_t skip = __builtin_popcount(mask & ((1u << (8 * q)) - 1u));
+        // the codes from the skip-th on.  (Not a shift of 64 bits: with its amount in the last vector register that a
+        // kernel has, this GPU shifts by something else now and then, and the compiler does not keep from it.)
+        return dequant_chunk_sparse(__builtin_amdgcn_alignbit(skip < 8 ? hi : 0u, skip < 8 ? lo : hi, 4 * skip), (mask >> (8 * q)) & 0xFFu, lut, co);
+    } else if constexpr (BITS == 4) {
+        return dequant_chunk<4>(lo, co);
+    } else if constexpr (BITS == 2) {
+        return dequant_chunk<2>(lo >> (16 * (q & 1)), co);
+    } else {
+        // bits 24 q ... 24 q + 23 of the 96
+        return dequant_chunk<3>(__builtin_amdgcn_alignbit(q == 3 ? 0u : hi, q == 3 ? hi : lo, (32 - 8 * q) & 31), co);
+    }
+}
+// a lane's first packed row of a 32-row block; int3 and 16:32 load the next one too
+template <int BITS, bool SPARSE>
+__device__ __forceinline__ uint32_t packed_row(int q) { return BITS == 4 && !SPARSE ? q : BITS == 2 ? q >> 1 : BITS == 3 ? (q > 0 ? q - 1 : 0) : 0; }
+template <int BITS, bool SPARSE>
+__device__ __forceinline__ uint32_t packed_row2(int q) { return SPARSE ? 1u : min(packed_row<BITS, SPARSE>(q) + 1u, 2u); }
+
+// (A, B) of sum x w = A sum x value + B sum x
+template <bool SPARSE>
+__device__ __forceinline__ void fold_factors(uint32_t s2, uint32_t z2, int odd, float& A, float& B) {
+    const float s = (float)as_h2(s2)[odd], z = (float)as_h2(z2)[odd];
+    const bool linear = s >= 0.f;
+    A = linear ? s : SPARSE ? 1.f : -s;
+    B = linear ? -s * z : z;
+}
+// a negative or NaN scale anywhere in the wave: the decode that serves either mode
+__device__ __forceinline__ bool any_negative(uint32_t a, uint32_t b) { return __builtin_amdgcn_ballot_w64(((a | b) & 0x80008000u) != 0) != 0; }
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);        // raw, 32-bit data format
+}
+__device__ __forceinline__ void fill_lut(uint32_t* lut, int t, int threads) {
+    for (int e = t; e < 256; e += threads) {
+        uint32_t v[8];
+        sparse_lut_entry(e, v);
+        *reinterpret_cast<u32x4*>(lut + e * 8) = u32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<u32x4*>(lut + e * 8 + 4) = u32x4{v[4], v[5], v[6], v[7]};
+    }
+    __syncthreads();
+}
+
 // ---- a product of up to 16 MT pairs of one expert with 64 columns.  UP: 32 columns of the gate and the same 32 of the other
 // half; the source row of a pair is its token's, the result h.  Else: 64 columns, source and result by place.
 template <int BITS, bool SPARSE, int MT, int WAVES, int DEPTH, bool UP>
 __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(ExpertsArgs a) {
     using F = RowsFmt<BITS, SPARSE>;
-    constexpr int HEIGHT = 16 * MT, RSRC = 0x00020000;
+    constexpr int HEIGHT = 16 * MT;
     // sums of what the codes stand for, scale and zero once per group; tall blocks have no registers for it and round their weights
     constexpr bool VALUES = MT <= 2, SUM_X = VALUES && !SPARSE;
     __shared__ __attribute__((aligned(16))) float red[WAVES * HEIGHT * 64];
@@ -137,27 +185,18 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
     if (find_block(a.offsets, a.experts, HEIGHT, blockIdx.x / a.strips, lane, block) >= 0) return;
     const int expert = block.expert, first = block.first, count = block.count;
     const int strip = blockIdx.x % a.strips;
-    if constexpr (SPARSE) {
-        for (int e = t; e < 256; e += 64 * WAVES) {
-            uint32_t v[8];
-            sparse_lut_entry(e, v);
-            *reinterpret_cast<u32x4*>(lut + e * 8) = u32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<u32x4*>(lut + e * 8 + 4) = u32x4{v[4], v[5], v[6], v[7]};
-        }
-        __syncthreads();
-    }
+    if constexpr (SPARSE) fill_lut(lut, t, 64 * WAVES);
     const int half = a.S / 2;
     // lane n's four columns of the strip
     const int col = UP ? (n < 8 ? 0 : half - 32) + 32 * strip + 4 * n : 64 * strip + 4 * n;
     // every load is a buffer, an offset of the lane that does not change and a uniform one that moves with k
     const int units = a.K / 64, groups = (units + a.group_units - 1) / a.group_units;
     const uint32_t row_bytes = 4u * (uint32_t)a.S;
-    auto buffer = [](const void* p, uint32_t bytes) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, RSRC); };
-    const __amdgpu_buffer_rsrc_t w_rsrc = buffer(a.matrix + expert * a.matrix_stride, 2 * units * F::ROWS * row_bytes);
-    const __amdgpu_buffer_rsrc_t m_rsrc = buffer(SPARSE ? a.mask + expert * a.mask_stride : a.matrix, 2 * units * row_bytes);
-    const __amdgpu_buffer_rsrc_t s_rsrc = buffer(a.scales + expert * a.scale_stride, groups * (row_bytes / 2));
-    const __amdgpu_buffer_rsrc_t z_rsrc = buffer(a.zeros + expert * a.scale_stride, groups * (row_bytes / 2));
-    const __amdgpu_buffer_rsrc_t x_rsrc = UP ? buffer(a.x, a.x_bytes) : buffer(a.x + (int64_t)first * a.K, 2u * (uint32_t)count * a.K);
+    const __amdgpu_buffer_rsrc_t w_rsrc = buffer_of(a.matrix + expert * a.matrix_stride, 2 * units * F::ROWS * row_bytes);
+    const __amdgpu_buffer_rsrc_t m_rsrc = buffer_of(SPARSE ? a.mask + expert * a.mask_stride : a.matrix, 2 * units * row_bytes);
+    const __amdgpu_buffer_rsrc_t s_rsrc = buffer_of(a.scales + expert * a.scale_stride, groups * (row_bytes / 2));
+    const __amdgpu_buffer_rsrc_t z_rsrc = buffer_of(a.zeros + expert * a.scale_stride, groups * (row_bytes / 2));
+    const __amdgpu_buffer_rsrc_t x_rsrc = UP ? buffer_of(a.x, a.x_bytes) : buffer_of(a.x + (int64_t)first * a.K, 2u * (uint32_t)count * a.K);
     // states: eight lanes read the 128 bytes of a row (one lane for 16 bytes of every row, as the operands want them, are 64 accesses of
     // the L1 a load, four times as many), and the wave turns them in LDS of its own: chunk c of row r stands at c ^ (r % 8)
     uint32_t x_off[2 * MT];
@@ -169,8 +208,7 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
     // (written and read as the same type: without a barrier between, the compiler has to see that they are the same memory)
     char* const stage = staged + wave * (HEIGHT * 128);
     char* const stage_to = stage + (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16;
-    const uint32_t row0 = BITS == 4 && !SPARSE ? q : BITS == 2 ? q >> 1 : BITS == 3 ? (q > 0 ? q - 1 : 0) : 0;
-    const uint32_t w_off = 4u * col + row0 * row_bytes, w_off2 = 4u * col + (SPARSE ? 1 : min(row0 + 1, 2u)) * row_bytes;
+    const uint32_t w_off = 4u * col + packed_row<BITS, SPARSE>(q) * row_bytes, w_off2 = 4u * col + packed_row2<BITS, SPARSE>(q) * row_bytes;
 
     struct Unit {                                     // 64 k
         u32x4 w[2][F::LOADS];
@@ -219,23 +257,7 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
             co.set(as_h2(__builtin_amdgcn_perm(u.s[j >> 1], u.s[j >> 1], sel)), as_h2(__builtin_amdgcn_perm(u.z[j >> 1], u.z[j >> 1], sel)));
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                h16x8 w;
-                if constexpr (SPARSE) {
-                    const uint32_t m = u.w[b][2][j], m8 = (m >> (8 * q)) & 0xFFu;
-                    const uint32_t skip = __builtin_popcount(m & ((1u << (8 * q)) - 1u));
-                    // the codes from the skip-th on.  (Not a shift of 64 bits: with its amount in the last vector register that a
-                    // kernel has, this GPU shifts by something else now and then, and the compiler does not keep from it.)
-                    const uint32_t lo = u.w[b][0][j], hi = u.w[b][1][j];
-                    w = dequant_chunk_sparse(__builtin_amdgcn_alignbit(skip < 8 ? hi : 0u, skip < 8 ? lo : hi, 4 * skip), m8, lut, co);
-                } else if constexpr (BITS == 4) {
-                    w = dequant_chunk<4>(u.w[b][0][j], co);
-                } else if constexpr (BITS == 2) {
-                    w = dequant_chunk<2>(u.w[b][0][j] >> (16 * (q & 1)), co);
-                } else {
-                    // bits 24 q ... 24 q + 23 of the 96
-                    const uint32_t lo = u.w[b][0][j], hi = u.w[b][1][j];
-                    w = dequant_chunk<3>(__builtin_amdgcn_alignbit(q == 3 ? 0u : hi, q == 3 ? hi : lo, (32 - 8 * q) & 31), co);
-                }
+                const h16x8 w = operand_of<BITS, SPARSE>(u.w[b][0][j], F::LOADS > 1 ? u.w[b][F::LOADS > 1][j] : 0u, F::LOADS > 2 ? u.w[b][F::LOADS - 1][j] : 0u, q, lut, co);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[b][m], w, acc[m][j], 0, 0, 0);
             }
@@ -252,9 +274,8 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
     auto fold = [&](const Unit& u) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float s = (float)as_h2(u.s[j >> 1])[j & 1], z = (float)as_h2(u.z[j >> 1])[j & 1];
-            const bool linear = s >= 0.f;
-            const float A = SPARSE ? (linear ? s : 1.f) : linear ? s : -s, B = linear ? -s * z : z;
+            float A, B;
+            fold_factors<SPARSE>(u.s[j >> 1], u.z[j >> 1], j & 1, A, B);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -292,9 +313,7 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
                 load_x(min(i + d + 1, u1 - 1));
                 __builtin_amdgcn_sched_barrier(0);
                 if (i + d < u1) {
-                    // a negative or NaN scale anywhere in the wave: the decode that serves either mode
-                    const bool negative = __builtin_amdgcn_ballot_w64(((now.s[0] | now.s[1]) & 0x80008000u) != 0) != 0;
-                    if ((VALUES || BITS == 4) && negative) multiply(std::bool_constant<VALUES || BITS == 4>{}, now);
+                    if ((VALUES || BITS == 4) && any_negative(now.s[0], now.s[1])) multiply(std::bool_constant<VALUES || BITS == 4>{}, now);
                     else multiply(std::false_type{}, now);
                     if constexpr (VALUES) {
                         if (--left == 0 || i + d == u1 - 1) {
@@ -334,6 +353,149 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
         } else {
             *reinterpret_cast<f32x4*>(a.part + (int64_t)(first + row) * a.S + 64 * strip + c) = total(row, c);
         }
+    }
+}
+
+// ---- few pairs, hardly two of them of the same expert: no order, a workgroup takes a pair and 64 columns, two launches in all.
+// What bounds them at that size is latency and the issue of instructions.  The second product's workgroups of a token and a strip
+// store their weighted sums write-through and count themselves in, and the last to arrive adds them up in the order of the slots: a
+// sum of one order, whoever is last.  Measured, one token, eight of 64 experts of 2048 x 1024, a call: 14.5 us; with sixteen waves
+// 15.8; with all pairs of a token in one workgroup, as one long K, which leaves three quarters of the CUs idle, 18.4; through
+// plan_kernel, rows_kernel and combine_kernel 19.5.
+template <int BITS, bool SPARSE, bool UP>
+__global__ __launch_bounds__(512) void token_kernel(ExpertsArgs a) {
+    using F = RowsFmt<BITS, SPARSE>;
+    constexpr int WAVES = 8, DEPTH = 2, THROUGH = 17;        // THROUGH: sc0 | sc1, straight to memory
+    __shared__ __attribute__((aligned(16))) float red[WAVES * 64];
+    __shared__ __attribute__((aligned(16))) uint32_t lut[SPARSE ? SPARSE_LUT_WORDS : 4];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int n = lane & 15, q = lane >> 4, strip = blockIdx.x % a.strips, pair = blockIdx.x / a.strips;
+    const int token = pair / a.top_k, half = a.S / 2;
+    const int id = a.ids[pair];
+    const bool valid = (uint32_t)id < (uint32_t)a.experts;
+    if constexpr (UP) {
+        // the second product's counters, one for each of its strips of the token
+        if (strip == 0 && pair == token * a.top_k)
+            for (int c = t; c < a.K / 64; c += 64 * WAVES) a.arrivals[token * (a.K / 64) + c] = 0;
+        if (!valid) return;
+    }
+    const int col = UP ? (n < 8 ? 0 : half - 32) + 32 * strip + 4 * n : 64 * strip + 4 * n;
+    const int units = a.K / 64, groups = (units + a.group_units - 1) / a.group_units;
+    const uint32_t row_bytes = 4u * (uint32_t)a.S;
+    const int64_t e = valid ? id : 0;
+    const __amdgpu_buffer_rsrc_t w_rsrc = buffer_of(a.matrix + e * a.matrix_stride, 2 * units * F::ROWS * row_bytes);
+    const __amdgpu_buffer_rsrc_t m_rsrc = buffer_of(SPARSE ? a.mask + e * a.mask_stride : a.matrix, 2 * units * row_bytes);
+    const __amdgpu_buffer_rsrc_t s_rsrc = buffer_of(a.scales + e * a.scale_stride, groups * (row_bytes / 2));
+    const __amdgpu_buffer_rsrc_t z_rsrc = buffer_of(a.zeros + e * a.scale_stride, groups * (row_bytes / 2));
+    const __amdgpu_buffer_rsrc_t x_rsrc = buffer_of(a.x + (int64_t)(UP ? token : pair) * a.K, 2u * (uint32_t)a.K);
+    const uint32_t w_off = 4u * col + packed_row<BITS, SPARSE>(q) * row_bytes, w_off2 = 4u * col + packed_row2<BITS, SPARSE>(q) * row_bytes;
+    struct Unit {
+        u32x4 w[2][F::LOADS];
+        u32x4 x[2];
+        u32x2 s, z;
+    };
+    auto load = [&](Unit& u, int unit) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const uint32_t blk = (uint32_t)(2 * unit + b) * row_bytes;
+            u.w[b][0] = __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, w_off, blk * F::ROWS, 0);
+            if constexpr (F::LOADS > 1) u.w[b][1] = __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, w_off2, blk * F::ROWS, 0);
+            if constexpr (SPARSE) u.w[b][2] = __builtin_amdgcn_raw_buffer_load_b128(m_rsrc, 4u * col, blk, 0);
+            // (all rows of the operand are the one row)
+            u.x[b] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, 16u * q, 128u * unit + 64u * b, 0);
+        }
+        const uint32_t g = (uint32_t)magic_div(unit, a.group_units, a.group_magic) * (row_bytes / 2);
+        u.s = __builtin_amdgcn_raw_buffer_load_b64(s_rsrc, 2u * col, g, 0);
+        u.z = __builtin_amdgcn_raw_buffer_load_b64(z_rsrc, 2u * col, g, 0);
+    };
+    f32x4 acc[4], acc_x;
+    float sum[4];
+    auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        acc_x = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    clear();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = 0.f;
+    const h16x8 ones = bitcast<h16x8>(u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
+    auto multiply = [&](auto mode, const Unit& u) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            Values<BITS, SPARSE, decltype(mode)::value> co;
+            const uint32_t sel = (j & 1) ? 0x03020302u : 0x01000100u;
+            co.set(as_h2(__builtin_amdgcn_perm(u.s[j >> 1], u.s[j >> 1], sel)), as_h2(__builtin_amdgcn_perm(u.z[j >> 1], u.z[j >> 1], sel)));
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const h16x8 w = operand_of<BITS, SPARSE>(u.w[b][0][j], F::LOADS > 1 ? u.w[b][F::LOADS > 1][j] : 0u, F::LOADS > 2 ? u.w[b][F::LOADS - 1][j] : 0u, q, lut, co);
+                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<h16x8>(u.x[b]), w, acc[j], 0, 0, 0);
+            }
+        }
+        if constexpr (!SPARSE) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) acc_x = __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<h16x8>(u.x[b]), ones, acc_x, 0, 0, 0);
+        }
+    };
+    const int u0 = units * wave / WAVES, u1 = valid ? units * (wave + 1) / WAVES : u0;
+    Unit ring[DEPTH];
+    if (u0 < u1) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            load(ring[d], min(u0 + d, u1 - 1));
+            __builtin_amdgcn_sched_barrier(0);        // (in this order, which the waits in the loop go by)
+        }
+    }
+    if constexpr (SPARSE) fill_lut(lut, t, 64 * WAVES);
+    if (u0 < u1) {
+        int left = a.group_units - (u0 - magic_div(u0, a.group_units, a.group_magic) * a.group_units);
+#pragma unroll 1
+        for (int i = u0; i < u1; i += DEPTH) {
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                const Unit& now = ring[d];
+                if (i + d < u1) {
+                    if (any_negative(now.s[0], now.s[1])) multiply(std::true_type{}, now);
+                    else multiply(std::false_type{}, now);
+                    if (--left == 0 || i + d == u1 - 1) {         // the end of a group or of the wave's part
+                        left = a.group_units;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float A, B;
+                            fold_factors<SPARSE>(now.s[j >> 1], now.z[j >> 1], j & 1, A, B);
+                            if constexpr (!SPARSE) sum[j] = fmaf(B, acc_x[0], sum[j]);
+                            sum[j] = fmaf(A, acc[j][0], sum[j]);
+                        }
+                        clear();
+                    }
+                }
+                load(ring[d], min(i + d + DEPTH, u1 - 1));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+    if (q == 0) *reinterpret_cast<f32x4*>(red + wave * 64 + 4 * n) = f32x4{sum[0], sum[1], sum[2], sum[3]};
+    __syncthreads();
+    auto total = [&](int c) __attribute__((always_inline)) {
+        float s = red[c];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) s += red[w * 64 + c];
+        return s;
+    };
+    if constexpr (UP) {
+        if (t < 32) a.h[(int64_t)pair * half + 32 * strip + t] = (h16)silu_times(total(t), total(t + 32));
+    } else {
+        if (wave != 0) return;
+        const int slot = pair - token * a.top_k;
+        const __amdgpu_buffer_rsrc_t parts = buffer_of(a.part + ((int64_t)token * a.strips + strip) * a.top_k * 64, a.top_k * 256);
+        const float v = valid ? a.weights[pair] * total(t) : 0.f;
+        __builtin_amdgcn_raw_buffer_store_b32(bitcast<uint32_t>(v), parts, 256u * slot + 4u * t, 0, THROUGH);
+        __builtin_amdgcn_s_waitcnt(0);                // every store of the wave has been acknowledged
+        int arrived = 0;
+        if (t == 0) arrived = __hip_atomic_fetch_add(a.arrivals + token * a.strips + strip, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (__builtin_amdgcn_readfirstlane(arrived) != a.top_k - 1) return;
+        float s = 0.f;
+        for (int j = 0; j < a.top_k; ++j) s += bitcast<float>(__builtin_amdgcn_raw_buffer_load_b32(parts, 256u * j + 4u * t, 0, THROUGH));
+        a.outs[(int64_t)token * a.S + 64 * strip + t] = (h16)s;
     }
 }
 
@@ -380,6 +542,16 @@ static void rows_product(int bits, const ExpertsArgs& a, int mt, int64_t pairs, 
     else launch_rows<2, false, UP>(a, mt, pairs, st);
 }
 
+template <bool UP>
+static void token_product(int bits, ExpertsArgs a, int64_t pairs, hipStream_t st) {
+    a.strips = a.S / 64;
+    const dim3 grid((unsigned)(pairs * a.strips)), block(512);
+    if (a.mask) hipLaunchKernelGGL((token_kernel<4, true, UP>), grid, block, 0, st, a);
+    else if (bits == 4) hipLaunchKernelGGL((token_kernel<4, false, UP>), grid, block, 0, st, a);
+    else if (bits == 3) hipLaunchKernelGGL((token_kernel<3, false, UP>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((token_kernel<2, false, UP>), grid, block, 0, st, a);
+}
+
 static int check_experts(int bits, const int4mm_experts_shape* sh, bool sparse) {
     if (sh == nullptr) return INT4MM_ERR_NULL;
     if (bits != 4 && bits != 3 && bits != 2) return INT4MM_ERR_BITS;
@@ -398,7 +570,7 @@ static int check_experts(int bits, const int4mm_experts_shape* sh, bool sparse) 
     return INT4MM_OK;
 }
 
-struct ExpertsParts { size_t offsets, order, place, h, part, total; };
+struct ExpertsParts { size_t offsets, order, place, arrivals, h, part, total; };
 static ExpertsParts experts_parts(const int4mm_experts_shape& sh) {
     const size_t pairs = (size_t)(sh.tokens * sh.top_k);
     auto round = [](size_t n) { return (n + 255) & ~size_t(255); };
@@ -406,7 +578,8 @@ static ExpertsParts experts_parts(const int4mm_experts_shape& sh) {
     p.offsets = 0;
     p.order = p.offsets + round(4 * (size_t)(sh.experts + 1));
     p.place = p.order + round(4 * pairs);
-    p.h = p.place + round(4 * pairs);
+    p.arrivals = p.place + round(4 * pairs);              // (pairs by themselves: up to 64 tokens)
+    p.h = p.arrivals + (pairs <= 64 ? round(4 * (size_t)(sh.tokens * (sh.in_size / 64))) : 0);
     p.part = p.h + round(2 * pairs * (size_t)sh.width);
     p.total = p.part + round(4 * pairs * (size_t)sh.in_size);
     return p;
@@ -449,12 +622,18 @@ int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weig
     a.order = reinterpret_cast<int*>(ws + parts.order);
     a.h = reinterpret_cast<h16*>(ws + parts.h);
     a.part = reinterpret_cast<float*>(ws + parts.part);
+    a.arrivals = reinterpret_cast<int*>(ws + parts.arrivals);
     a.experts = E;
     a.top_k = (int)sh->top_k;
     a.group_units = (int)(sh->group_size < 0 ? std::max(K, F) / 64 : std::min(sh->group_size, std::max(K, F) + 63) / 64);
     a.group_magic = div_magic((uint32_t)a.group_units);
-    hipLaunchKernelGGL(plan_kernel, dim3(E), dim3(1024), 0, st, static_cast<const int*>(ids), const_cast<int*>(a.offsets),
-                           const_cast<int*>(a.order), place, (int)pairs, E);
+    a.ids = static_cast<const int*>(ids);
+    a.weights = static_cast<const float*>(weights);
+    a.outs = static_cast<h16*>(outs);
+    // a pair by itself: one token, or so few pairs that hardly two of them share an expert
+    const bool single = pairs <= 64 && (sh->tokens == 1 || 2 * pairs <= E);
+    if (!single)
+        hipLaunchKernelGGL(plan_kernel, dim3(E), dim3(1024), 0, st, a.ids, const_cast<int*>(a.offsets), const_cast<int*>(a.order), place, (int)pairs, E);
     if (const int rc = check_launch("experts_forward")) return rc;
     // pairs per expert, if all are asked alike
     const int64_t mean = pairs / E;
@@ -473,7 +652,8 @@ int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weig
     a.mask_stride = K / 32 * 2 * F;
     a.scale_stride = sh->up_groups * 2 * F;
     a.x_bytes = (uint32_t)(sh->tokens * K * 2);
-    if (tiles) launch_experts_tiles(bits, a, tm, pairs, true, st);
+    if (single) token_product<true>(bits, a, pairs, st);
+    else if (tiles) launch_experts_tiles(bits, a, tm, pairs, true, st);
     else rows_product<true>(bits, a, mt, pairs, st);
     if (const int rc = check_launch("experts_forward")) return rc;
     a.x = a.h;
@@ -486,6 +666,10 @@ int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weig
     a.matrix_stride = rows_of(F) * K;
     a.mask_stride = F / 32 * K;
     a.scale_stride = sh->down_groups * K;
+    if (single) {
+        token_product<false>(bits, a, pairs, st);
+        return check_launch("experts_forward");
+    }
     if (tiles) {
         a.h = reinterpret_cast<h16*>(ws + parts.part);
         launch_experts_tiles(bits, a, tm, pairs, false, st);
@@ -496,11 +680,10 @@ int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weig
     const int columns = (int)((K + (tiles ? 2047 : 1023)) / (tiles ? 2048 : 1024));
     const dim3 grid((unsigned)(sh->tokens * columns));
     if (tiles)
-        hipLaunchKernelGGL(combine_kernel<h16>, grid, dim3(256), 0, st, static_cast<h16*>(outs), a.h, static_cast<const float*>(weights), place,
+        hipLaunchKernelGGL(combine_kernel<h16>, grid, dim3(256), 0, st, a.outs, a.h, a.weights, place,
                            a.top_k, (int)K, columns);
     else
-        hipLaunchKernelGGL(combine_kernel<float>, grid, dim3(256), 0, st, static_cast<h16*>(outs), a.part, static_cast<const float*>(weights),
-                           place, a.top_k, (int)K, columns);
+        hipLaunchKernelGGL(combine_kernel<float>, grid, dim3(256), 0, st, a.outs, a.part, a.weights, place, a.top_k, (int)K, columns);
     return check_launch("experts_forward");
 }
 
