@@ -56,7 +56,7 @@ __device__ __forceinline__ int find_block(const int* offsets, int experts, int h
     return before;
 }
 
-// experts_tiles.hip: both products in tiles of 32 tm rows (tm: 2, 4, 8) and 256 columns
+// experts_tiles.hip: both products in tiles of 32 tm rows (tm: 2, 3, 4, 6 or 8) and 256 columns
 void launch_experts_tiles(int bits, const ExpertsArgs& a, int tm, int64_t pairs, bool gated, hipStream_t st);
 
 }  // namespace i4

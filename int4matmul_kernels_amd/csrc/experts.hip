@@ -11,10 +11,9 @@
 // rows_kernel is bound by reading the packed weights and by the instructions that decode them.  The waves of a workgroup share K out,
 // so nothing is shared through LDS in the loop: a lane loads 16 bytes of packed words, four neighbouring columns of the packed row
 // that holds its 8 k, and each word is after its decode the operand of one v_mfma_f32_16x16x32_f16 whose columns are every fourth
-// of the strip.  Blocks of up to 32 pairs multiply what the codes stand for, exact in fp16, and apply scale and zero once per group
-// to the sums (sum x w = s (sum x q - z sum x), the sum of x from a product with ones), which takes 7 instructions a word where
-// rounded weights take 17 and is nearer to the exact product; 64 pairs have no registers for it and round their weights as the tile
-// kernels do.  The partial sums of the waves meet in LDS.
+// of the strip.  What is multiplied is what the codes stand for, exact in fp16; scale and zero are applied once per group to the sums
+// (sum x w = s (sum x q - z sum x), the sum of x from a product with ones), which takes 7 instructions a word where rounded weights
+// take 17 and is nearer to the exact product.  The partial sums of the waves meet in LDS.
 //
 // Measured (64 tokens, two of eight experts of 4096 x 11008, int4, us a call): weights rounded, addresses computed, one lane for 16
 // bytes of every row of states 198; exact codes, buffer loads, two units in flight in the order that the waits go by 178; states
@@ -22,6 +21,7 @@
 #include "experts.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace i4 {
 
@@ -171,11 +171,9 @@ __device__ __forceinline__ void fill_lut(uint32_t* lut, int t, int threads) {
 // ---- a product of up to 16 MT pairs of one expert with 64 columns.  UP: 32 columns of the gate and the same 32 of the other
 // half; the source row of a pair is its token's, the result h.  Else: 64 columns, source and result by place.
 template <int BITS, bool SPARSE, int MT, int WAVES, int DEPTH, bool UP>
-__global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(ExpertsArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 2) void rows_kernel(ExpertsArgs a) {
     using F = RowsFmt<BITS, SPARSE>;
     constexpr int HEIGHT = 16 * MT;
-    // sums of what the codes stand for, scale and zero once per group; tall blocks have no registers for it and round their weights
-    constexpr bool VALUES = MT <= 2, SUM_X = VALUES && !SPARSE;
     __shared__ __attribute__((aligned(16))) float red[WAVES * HEIGHT * 64];
     __shared__ __attribute__((aligned(16))) char staged[WAVES * HEIGHT * 128];
     __shared__ __attribute__((aligned(16))) uint32_t lut[SPARSE ? SPARSE_LUT_WORDS : 4];
@@ -227,7 +225,7 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
         u.z = __builtin_amdgcn_raw_buffer_load_b64(z_rsrc, 2u * col, g, 0);
     };
 
-    f32x4 acc[MT][4], acc_x[MT], sum[VALUES ? MT : 1][4];
+    f32x4 acc[MT][4], acc_x[MT], sum[MT][4];
     auto clear = [&](auto& v) __attribute__((always_inline)) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -240,10 +238,9 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
         for (int m = 0; m < MT; ++m) acc_x[m] = f32x4{0.f, 0.f, 0.f, 0.f};
     };
     clear_group();
-    if constexpr (VALUES) clear(sum);
+    clear(sum);
     const h16x8 ones = bitcast<h16x8>(u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
     auto multiply = [&](auto mode, const Unit& u) __attribute__((always_inline)) {
-        constexpr bool either = decltype(mode)::value;
         h16x8 x[2][MT];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -252,7 +249,7 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
                 x[b][m] = bitcast<h16x8>(*reinterpret_cast<const u32x4*>(stage + (16 * m + n) * 128 + (((4 * b + q) ^ n) & 7) * 16));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            std::conditional_t<VALUES, Values<BITS, SPARSE, either>, Coef<BITS, either>> co;
+            Values<BITS, SPARSE, decltype(mode)::value> co;
             const uint32_t sel = (j & 1) ? 0x03020302u : 0x01000100u;
             co.set(as_h2(__builtin_amdgcn_perm(u.s[j >> 1], u.s[j >> 1], sel)), as_h2(__builtin_amdgcn_perm(u.z[j >> 1], u.z[j >> 1], sel)));
 #pragma unroll
@@ -262,7 +259,7 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
                 for (int m = 0; m < MT; ++m) acc[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[b][m], w, acc[m][j], 0, 0, 0);
             }
         }
-        if constexpr (SUM_X) {
+        if constexpr (!SPARSE) {
             // (every column of this product is the rows' sums: a lane has those of the rows that it has results of)
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -280,7 +277,7 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if constexpr (SUM_X) sum[m][j][r] = fmaf(B, acc_x[m][r], sum[m][j][r]);
+                    if constexpr (!SPARSE) sum[m][j][r] = fmaf(B, acc_x[m][r], sum[m][j][r]);
                     sum[m][j][r] = fmaf(A, acc[m][j][r], sum[m][j][r]);
                 }
         }
@@ -313,13 +310,11 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
                 load_x(min(i + d + 1, u1 - 1));
                 __builtin_amdgcn_sched_barrier(0);
                 if (i + d < u1) {
-                    if ((VALUES || BITS == 4) && any_negative(now.s[0], now.s[1])) multiply(std::bool_constant<VALUES || BITS == 4>{}, now);
+                    if (any_negative(now.s[0], now.s[1])) multiply(std::true_type{}, now);
                     else multiply(std::false_type{}, now);
-                    if constexpr (VALUES) {
-                        if (--left == 0 || i + d == u1 - 1) {
-                            fold(now);
-                            left = a.group_units;
-                        }
+                    if (--left == 0 || i + d == u1 - 1) {
+                        fold(now);
+                        left = a.group_units;
                     }
                 }
                 load(ring[d], min(i + d + DEPTH, u1 - 1));
@@ -327,13 +322,12 @@ __global__ __launch_bounds__(64 * WAVES, MT == 4 ? 1 : 2) void rows_kernel(Exper
             }
         }
     }
-    auto& result = [&]() -> auto& { if constexpr (VALUES) return sum; else return acc; }();
     // register r of tile (m, j): row 16 m + 4 q + r, column 4 n + j of the strip
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            *reinterpret_cast<f32x4*>(red + (wave * HEIGHT + 16 * m + 4 * q + r) * 64 + 4 * n) = f32x4{result[m][0][r], result[m][1][r], result[m][2][r], result[m][3][r]};
+            *reinterpret_cast<f32x4*>(red + (wave * HEIGHT + 16 * m + 4 * q + r) * 64 + 4 * n) = f32x4{sum[m][0][r], sum[m][1][r], sum[m][2][r], sum[m][3][r]};
     __syncthreads();
     auto total = [&](int row, int c) __attribute__((always_inline)) {
         f32x4 s = *reinterpret_cast<const f32x4*>(red + row * 64 + c);
@@ -524,22 +518,62 @@ __global__ __launch_bounds__(256) void combine_kernel(h16* outs, const T* part, 
     *reinterpret_cast<Out*>(outs + t * S + c) = o;
 }
 
+// ---- which kernels, by the pairs of an expert if all are asked alike (the host does not know how they are shared out).
+//
+// A pair by itself: one token, or so few pairs that hardly two of them share an expert.
+//
+// Blocks of rows_kernel up to a mean of 40, then tiles.  us a call, 16 experts of 2048 x 1408, means of 8 / 32 / 48 / 64: blocks of
+// 32 pairs int4 36 / 50 / 60 / 70, int3 41 / 58 / 68 / 79, 16:32 47 / 66 / 78 / 92; tiles of 64 (and at 64: 96) rows int4 - / 56 / 56 / 58,
+// int3 - / 58 / 59 / 61, 16:32 - / 79 / 78 / 82.  Blocks of 64 pairs were slower than either everywhere.  Blocks of 16 pairs, of eight
+// waves: int4 at means of 4 / 8 / 12 30 / 34 / 36 where 32 take 36 / 36 / 36, but int3 40 / 45 / 51 and 41 / 41 / 41, 16:32 47 / 53 / 60 and
+// 48 / 47 / 46.
+//
+// The height of the tiles: rounds of 256 workgroups times what a K step takes, with the blocks that an expert is expected to need
+// (normal around the mean; the last step's length from the tile kernels' cost model, matmul.hip).  int4, means of 64 / 96 / 128 / 192 /
+// 256 / 384, 64 rows 81 / 83 / 102 / 132 / 179 / 228, 96: 58 / 76 / 91 / 113 / 146 / 205, 128: 62 / 65 / 98 / 104 / 128 / 170, 192: 70 / 73 / 77 /
+// 120 / 126 / 161, 256: 78 / 81 / 85 / 94 / 141 / 154.
+constexpr bool low_blocks(int bits, bool sparse) { return bits != 3 && !sparse; }
+struct ExpertsPlan { bool single; int height; int tm; };         // tm: 0 (rows_kernel with blocks of `height` pairs) or tiles of 32 tm rows
+static ExpertsPlan plan_experts(int bits, bool sparse, const int4mm_experts_shape& sh) {
+    const int64_t pairs = sh.tokens * sh.top_k;
+    const double mean = (double)pairs / sh.experts;
+    ExpertsPlan p{pairs <= 64 && (sh.tokens == 1 || 2 * pairs <= sh.experts), low_blocks(bits, sparse) && mean <= 8 ? 16 : 32, 0};
+    if (p.single || mean <= 40) return p;
+    const double step[] = {0.30, 0.335, 0.373, 0.466, 0.555}, strips = (double)((sh.width + 127) / 128);
+    const int tms[] = {2, 3, 4, 6, 8};
+    double best = 1e30;
+    for (int i = 0; i < 5; ++i) {
+        const int h = 32 * tms[i];
+        // E ceil(c / h) = 1 + sum over n >= 1 of P(c > n h), which is 1 for the first of them
+        const double deviation = std::sqrt(mean);
+        int64_t n = std::max<int64_t>(1, (int64_t)((mean - 4 * deviation) / h));
+        double blocks = (double)n;
+        for (; n * h < mean + 4 * deviation; ++n) blocks += 0.5 * std::erfc((n * h - mean) / (deviation * 1.41421356));
+        const double rounds = sh.experts * blocks * strips / 256.0;
+        const double us = (rounds < 8 ? std::ceil(rounds) : rounds + 0.5) * step[i];
+        if (us < best) best = us, p.tm = tms[i];
+    }
+    return p;
+}
+
 template <int BITS, bool SPARSE, bool UP>
-static void launch_rows(ExpertsArgs a, int mt, int64_t pairs, hipStream_t st) {
+static void launch_rows(ExpertsArgs a, int height, int64_t pairs, hipStream_t st) {
     a.strips = a.S / 64;
-    const int64_t height = 16 * mt, blocks = std::min<int64_t>(pairs, a.experts + pairs / height);
-    const dim3 grid((unsigned)(blocks * a.strips));
-    if (mt == 1) hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 1, 8, 2, UP>), grid, dim3(512), 0, st, a);
-    else if (mt == 2) hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 2, 4, 2, UP>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 4, 4, 2, UP>), grid, dim3(256), 0, st, a);
+    const dim3 grid((unsigned)(std::min<int64_t>(pairs, a.experts + pairs / height) * a.strips));
+    if constexpr (low_blocks(BITS, SPARSE))
+        if (height == 16) {
+            hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 1, 8, 2, UP>), grid, dim3(512), 0, st, a);
+            return;
+        }
+    hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 2, 4, 2, UP>), grid, dim3(256), 0, st, a);
 }
 
 template <bool UP>
-static void rows_product(int bits, const ExpertsArgs& a, int mt, int64_t pairs, hipStream_t st) {
-    if (a.mask) launch_rows<4, true, UP>(a, mt, pairs, st);
-    else if (bits == 4) launch_rows<4, false, UP>(a, mt, pairs, st);
-    else if (bits == 3) launch_rows<3, false, UP>(a, mt, pairs, st);
-    else launch_rows<2, false, UP>(a, mt, pairs, st);
+static void rows_product(int bits, const ExpertsArgs& a, int height, int64_t pairs, hipStream_t st) {
+    if (a.mask) launch_rows<4, true, UP>(a, height, pairs, st);
+    else if (bits == 4) launch_rows<4, false, UP>(a, height, pairs, st);
+    else if (bits == 3) launch_rows<3, false, UP>(a, height, pairs, st);
+    else launch_rows<2, false, UP>(a, height, pairs, st);
 }
 
 template <bool UP>
@@ -552,37 +586,116 @@ static void token_product(int bits, ExpertsArgs a, int64_t pairs, hipStream_t st
     else hipLaunchKernelGGL((token_kernel<2, false, UP>), grid, block, 0, st, a);
 }
 
+// Tokens that go through the launches at once, in even shares: their states are addressed with 31 bits, and of many pairs (a quarter
+// of a million fill the GPU many times over) not all need a workspace at the same time.
+static int64_t tokens_at_once(const int4mm_experts_shape& sh) {
+    const int64_t most = std::max<int64_t>(1, std::min((((int64_t)1 << 31) - 1) / (2 * sh.in_size), ((int64_t)1 << 18) / sh.top_k));
+    const int64_t shares = (sh.tokens + most - 1) / most;
+    return shares <= 1 ? sh.tokens : (sh.tokens + shares - 1) / shares;
+}
+
 static int check_experts(int bits, const int4mm_experts_shape* sh, bool sparse) {
     if (sh == nullptr) return INT4MM_ERR_NULL;
     if (bits != 4 && bits != 3 && bits != 2) return INT4MM_ERR_BITS;
     if (sparse && bits != 4) return INT4MM_ERR_SPARSE_BITS;
     const int64_t limit = (int64_t)1 << 31, K = sh->in_size, F = sh->width, g = sh->group_size;
-    if (sh->tokens < 0 || sh->top_k < 1 || sh->experts < 1 || sh->experts > 65536 || K <= 0 || F <= 0 || K % 64 != 0 || F % 64 != 0) return INT4MM_ERR_SHAPE;
+    if (sh->tokens < 0 || sh->top_k < 1 || sh->experts < 1 || sh->experts > 4096 || K <= 0 || F <= 0 || K % 64 != 0 || F % 64 != 0) return INT4MM_ERR_SHAPE;
     if (g == 0 || (g > 0 && g % 64 != 0)) return INT4MM_ERR_GROUP;
     const int64_t up_groups = g < 0 ? 1 : (K + g - 1) / g, down_groups = g < 0 ? 1 : (F + g - 1) / g;
     if (sh->up_groups != up_groups || sh->down_groups != down_groups) return INT4MM_ERR_SHAPE;
     // (a matrix, and the rows of a block, are addressed with 31 bits)
     if (K >= limit / 128 || F >= limit / 128 || K * F >= limit) return INT4MM_ERR_SHAPE;
-    // (grids of one dimension: a workgroup per 16 pairs or expert and 64 columns)
-    if (sh->top_k > 1024 || sh->tokens > limit || (sh->tokens * sh->top_k / 16 + sh->experts) * (std::max(K, 2 * F) / 64) >= limit ||
-        sh->tokens * sh->top_k >= limit / 2)
-        return INT4MM_ERR_SHAPE;
+    if (sh->top_k > 1024 || sh->tokens >= limit) return INT4MM_ERR_SHAPE;
+    // (a grid of one dimension has a workgroup for every 16 pairs, or expert, and 64 columns)
+    if ((tokens_at_once(*sh) * sh->top_k / 16 + sh->experts) * (std::max(K, 2 * F) / 64) >= limit) return INT4MM_ERR_SHAPE;
     return INT4MM_OK;
 }
 
 struct ExpertsParts { size_t offsets, order, place, arrivals, h, part, total; };
 static ExpertsParts experts_parts(const int4mm_experts_shape& sh) {
-    const size_t pairs = (size_t)(sh.tokens * sh.top_k);
+    const int64_t tokens = tokens_at_once(sh);
+    const size_t pairs = (size_t)(tokens * sh.top_k);
     auto round = [](size_t n) { return (n + 255) & ~size_t(255); };
     ExpertsParts p;
     p.offsets = 0;
     p.order = p.offsets + round(4 * (size_t)(sh.experts + 1));
     p.place = p.order + round(4 * pairs);
     p.arrivals = p.place + round(4 * pairs);              // (pairs by themselves: up to 64 tokens)
-    p.h = p.arrivals + (pairs <= 64 ? round(4 * (size_t)(sh.tokens * (sh.in_size / 64))) : 0);
+    p.h = p.arrivals + (pairs <= 64 ? round(4 * (size_t)(tokens * (sh.in_size / 64))) : 0);
     p.part = p.h + round(2 * pairs * (size_t)sh.width);
     p.total = p.part + round(4 * pairs * (size_t)sh.in_size);
     return p;
+}
+
+static int experts_share(int bits, bool sparse, h16* outs, const h16* x, const float* weights, const int* ids, const void* up_matrix,
+                         const void* up_scales, const void* up_zeros, const void* up_mask, const void* down_matrix, const void* down_scales,
+                         const void* down_zeros, const void* down_mask, const int4mm_experts_shape* sh, const ExpertsParts& parts, char* ws,
+                         hipStream_t st) {
+    const int64_t pairs = sh->tokens * sh->top_k, K = sh->in_size, F = sh->width;
+    const int E = (int)sh->experts;
+    int* const place = reinterpret_cast<int*>(ws + parts.place);
+    ExpertsArgs a;
+    a.offsets = reinterpret_cast<int*>(ws + parts.offsets);
+    a.order = reinterpret_cast<int*>(ws + parts.order);
+    a.h = reinterpret_cast<h16*>(ws + parts.h);
+    a.part = reinterpret_cast<float*>(ws + parts.part);
+    a.arrivals = reinterpret_cast<int*>(ws + parts.arrivals);
+    a.experts = E;
+    a.top_k = (int)sh->top_k;
+    a.group_units = (int)(sh->group_size < 0 ? std::max(K, F) / 64 : std::min(sh->group_size, std::max(K, F) + 63) / 64);
+    a.group_magic = div_magic((uint32_t)a.group_units);
+    a.ids = ids;
+    a.weights = weights;
+    a.outs = outs;
+    const ExpertsPlan plan = plan_experts(bits, sparse, *sh);
+    if (!plan.single)
+        hipLaunchKernelGGL(plan_kernel, dim3(E), dim3(1024), 0, st, a.ids, const_cast<int*>(a.offsets), const_cast<int*>(a.order), place, (int)pairs, E);
+    if (const int rc = check_launch("experts_forward")) return rc;
+    auto rows_of = [&](int64_t k) { return sparse ? k / 16 : k * bits / 32; };
+    a.x = x;
+    a.matrix = static_cast<const uint32_t*>(up_matrix);
+    a.mask = static_cast<const uint32_t*>(up_mask);
+    a.scales = static_cast<const h16*>(up_scales);
+    a.zeros = static_cast<const h16*>(up_zeros);
+    a.K = (int)K;
+    a.S = (int)(2 * F);
+    a.matrix_stride = rows_of(K) * 2 * F;
+    a.mask_stride = K / 32 * 2 * F;
+    a.scale_stride = sh->up_groups * 2 * F;
+    a.x_bytes = (uint32_t)(sh->tokens * K * 2);
+    if (plan.single) token_product<true>(bits, a, pairs, st);
+    else if (plan.tm) launch_experts_tiles(bits, a, plan.tm, pairs, true, st);
+    else rows_product<true>(bits, a, plan.height, pairs, st);
+    if (const int rc = check_launch("experts_forward")) return rc;
+    a.x = a.h;
+    a.matrix = static_cast<const uint32_t*>(down_matrix);
+    a.mask = static_cast<const uint32_t*>(down_mask);
+    a.scales = static_cast<const h16*>(down_scales);
+    a.zeros = static_cast<const h16*>(down_zeros);
+    a.K = (int)F;
+    a.S = (int)K;
+    a.matrix_stride = rows_of(F) * K;
+    a.mask_stride = F / 32 * K;
+    a.scale_stride = sh->down_groups * K;
+    if (plan.single) {
+        token_product<false>(bits, a, pairs, st);
+        return check_launch("experts_forward");
+    }
+    if (plan.tm) {
+        a.h = reinterpret_cast<h16*>(ws + parts.part);
+        launch_experts_tiles(bits, a, plan.tm, pairs, false, st);
+    } else {
+        rows_product<false>(bits, a, plan.height, pairs, st);
+    }
+    if (const int rc = check_launch("experts_forward")) return rc;
+    const int columns = (int)((K + (plan.tm ? 2047 : 1023)) / (plan.tm ? 2048 : 1024));
+    const dim3 grid((unsigned)(sh->tokens * columns));
+    if (plan.tm)
+        hipLaunchKernelGGL(combine_kernel<h16>, grid, dim3(256), 0, st, a.outs, a.h, a.weights, place,
+                           a.top_k, (int)K, columns);
+    else
+        hipLaunchKernelGGL(combine_kernel<float>, grid, dim3(256), 0, st, a.outs, a.part, a.weights, place, a.top_k, (int)K, columns);
+    return check_launch("experts_forward");
 }
 
 }  // namespace i4
@@ -592,7 +705,7 @@ using namespace i4;
 extern "C" {
 
 size_t int4mm_experts_workspace_bytes(const int4mm_experts_shape* sh) {
-    if (sh == nullptr || sh->tokens <= 0 || sh->top_k <= 0 || sh->experts <= 0 || sh->width <= 0 || sh->in_size <= 0) return 0;
+    if (check_experts(4, sh, false) != INT4MM_OK || sh->tokens == 0) return 0;
     return experts_parts(*sh).total;
 }
 
@@ -612,79 +725,17 @@ int int4mm_experts_forward(int bits, void* outs, const void* x, const void* weig
     if ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(ids)) & 3) return INT4MM_ERR_ALIGN;
     const ExpertsParts parts = experts_parts(*sh);
     if (workspace == nullptr || workspace_bytes < parts.total) return INT4MM_ERR_WORKSPACE;
-    char* const ws = static_cast<char*>(workspace);
-    const int64_t pairs = sh->tokens * sh->top_k, K = sh->in_size, F = sh->width;
-    const int E = (int)sh->experts;
-    hipStream_t st = (hipStream_t)stream;
-    int* const place = reinterpret_cast<int*>(ws + parts.place);
-    ExpertsArgs a;
-    a.offsets = reinterpret_cast<int*>(ws + parts.offsets);
-    a.order = reinterpret_cast<int*>(ws + parts.order);
-    a.h = reinterpret_cast<h16*>(ws + parts.h);
-    a.part = reinterpret_cast<float*>(ws + parts.part);
-    a.arrivals = reinterpret_cast<int*>(ws + parts.arrivals);
-    a.experts = E;
-    a.top_k = (int)sh->top_k;
-    a.group_units = (int)(sh->group_size < 0 ? std::max(K, F) / 64 : std::min(sh->group_size, std::max(K, F) + 63) / 64);
-    a.group_magic = div_magic((uint32_t)a.group_units);
-    a.ids = static_cast<const int*>(ids);
-    a.weights = static_cast<const float*>(weights);
-    a.outs = static_cast<h16*>(outs);
-    // a pair by itself: one token, or so few pairs that hardly two of them share an expert
-    const bool single = pairs <= 64 && (sh->tokens == 1 || 2 * pairs <= E);
-    if (!single)
-        hipLaunchKernelGGL(plan_kernel, dim3(E), dim3(1024), 0, st, a.ids, const_cast<int*>(a.offsets), const_cast<int*>(a.order), place, (int)pairs, E);
-    if (const int rc = check_launch("experts_forward")) return rc;
-    // pairs per expert, if all are asked alike
-    const int64_t mean = pairs / E;
-    const int mt = mean <= 8 ? 1 : mean <= 24 ? 2 : 4;
-    const bool tiles = mean >= 64;
-    const int tm = mean < 96 ? 2 : mean < 256 ? 4 : 8;
-    auto rows_of = [&](int64_t k) { return sparse ? k / 16 : k * bits / 32; };
-    a.x = static_cast<const h16*>(x);
-    a.matrix = static_cast<const uint32_t*>(up_matrix);
-    a.mask = static_cast<const uint32_t*>(up_mask);
-    a.scales = static_cast<const h16*>(up_scales);
-    a.zeros = static_cast<const h16*>(up_zeros);
-    a.K = (int)K;
-    a.S = (int)(2 * F);
-    a.matrix_stride = rows_of(K) * 2 * F;
-    a.mask_stride = K / 32 * 2 * F;
-    a.scale_stride = sh->up_groups * 2 * F;
-    a.x_bytes = (uint32_t)(sh->tokens * K * 2);
-    if (single) token_product<true>(bits, a, pairs, st);
-    else if (tiles) launch_experts_tiles(bits, a, tm, pairs, true, st);
-    else rows_product<true>(bits, a, mt, pairs, st);
-    if (const int rc = check_launch("experts_forward")) return rc;
-    a.x = a.h;
-    a.matrix = static_cast<const uint32_t*>(down_matrix);
-    a.mask = static_cast<const uint32_t*>(down_mask);
-    a.scales = static_cast<const h16*>(down_scales);
-    a.zeros = static_cast<const h16*>(down_zeros);
-    a.K = (int)F;
-    a.S = (int)K;
-    a.matrix_stride = rows_of(F) * K;
-    a.mask_stride = F / 32 * K;
-    a.scale_stride = sh->down_groups * K;
-    if (single) {
-        token_product<false>(bits, a, pairs, st);
-        return check_launch("experts_forward");
+    const int64_t share = tokens_at_once(*sh), K = sh->in_size, k = sh->top_k;
+    for (int64_t t = 0; t < sh->tokens; t += share) {
+        int4mm_experts_shape part = *sh;
+        part.tokens = std::min(share, sh->tokens - t);
+        if (const int rc = experts_share(bits, sparse, static_cast<h16*>(outs) + t * K, static_cast<const h16*>(x) + t * K,
+                                         static_cast<const float*>(weights) + t * k, static_cast<const int*>(ids) + t * k, up_matrix, up_scales,
+                                         up_zeros, up_mask, down_matrix, down_scales, down_zeros, down_mask, &part, parts,
+                                         static_cast<char*>(workspace), (hipStream_t)stream))
+            return rc;
     }
-    if (tiles) {
-        a.h = reinterpret_cast<h16*>(ws + parts.part);
-        launch_experts_tiles(bits, a, tm, pairs, false, st);
-    } else {
-        rows_product<false>(bits, a, mt, pairs, st);
-    }
-    if (const int rc = check_launch("experts_forward")) return rc;
-    const int columns = (int)((K + (tiles ? 2047 : 1023)) / (tiles ? 2048 : 1024));
-    const dim3 grid((unsigned)(sh->tokens * columns));
-    if (tiles)
-        hipLaunchKernelGGL(combine_kernel<h16>, grid, dim3(256), 0, st, a.outs, a.h, a.weights, place,
-                           a.top_k, (int)K, columns);
-    else
-        hipLaunchKernelGGL(combine_kernel<float>, grid, dim3(256), 0, st, a.outs, a.part, a.weights, place, a.top_k, (int)K, columns);
-    return check_launch("experts_forward");
+    return INT4MM_OK;
 }
 
 }  // extern "C"

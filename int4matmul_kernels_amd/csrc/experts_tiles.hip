@@ -48,6 +48,8 @@ static void launch_height(ExpertsArgs a, int tm, int64_t pairs, hipStream_t st) 
     const int64_t blocks = std::min<int64_t>(pairs, a.experts + pairs / (32 * tm));
     const dim3 grid((unsigned)((blocks * a.strips + 7) / 8 * 8));
     if (tm == 2) hipLaunchKernelGGL((experts_tile_kernel<BITS, SPARSE, 2, GATED>), grid, dim3(512), 0, st, a);
+    else if (tm == 3) hipLaunchKernelGGL((experts_tile_kernel<BITS, SPARSE, 3, GATED>), grid, dim3(512), 0, st, a);
+    else if (tm == 6) hipLaunchKernelGGL((experts_tile_kernel<BITS, SPARSE, 6, GATED>), grid, dim3(512), 0, st, a);
     else if (tm == 4) hipLaunchKernelGGL((experts_tile_kernel<BITS, SPARSE, 4, GATED>), grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((experts_tile_kernel<BITS, SPARSE, 8, GATED>), grid, dim3(512), 0, st, a);
 }

@@ -51,7 +51,7 @@ def test_experts_arguments():
     assert call(tokens=0) == 0
     assert call(bits=5) == 1 and call(bits=3, masks=(OK, OK)) == 2
     for change in (dict(tokens=-1), dict(top_k=0), dict(experts=0), dict(in_size=96), dict(width=96), dict(width=0), dict(up_groups=3), dict(down_groups=3),
-                   dict(experts=65537), dict(tokens=1 << 40), dict(top_k=1025), dict(in_size=1 << 32), dict(tokens=1 << 29, top_k=8)):
+                   dict(experts=4097), dict(tokens=1 << 31), dict(top_k=1025), dict(in_size=1 << 32), dict(in_size=1 << 16, width=1 << 15)):
         assert call(**change) == 3, change
     for g in (0, 32, 96):
         sh = capi.experts_shape(4, 2, 8, 256, 128, 64)
