@@ -10,6 +10,11 @@
 //
 // h is split into two halves of 11 bits each, after scaling its row by a power of two to 512 ... 1024, so that nothing overflows
 // and 22 bits of it are multiplied: both products are on v_mfma_f32_16x16x32_f16, which are few beside the memory traffic.
+//
+// What bounds it: prompts, the traffic of base and outs (4096 rows, K=5120, S=20480, rank 16: 377 MB in 83 - 87 us, 4.4 TB/s, of which
+// expand_kernel 72; a large copy does 4.9); requests with an adapter each, reading the factors (64 of rank 64: 164 MB in 48 us, expand_kernel
+// 40 at 3.3 TB/s); small calls, two launches (one row 8 us; 777 rows of 24 adapters 23).  Rows of base and outs go through buffers whose
+// lanes lie beyond where a row is not the workgroup's: with conditions around loads and stores instead 4096 rows took 98.
 #include "common.h"
 
 #include <algorithm>
@@ -330,19 +335,20 @@ __global__ __launch_bounds__(256) void expand_kernel(AdapterArgs a) {
 
 struct AdapterPlan { int mt, nt, ksplit, units_per_split, deal_shrink, deal_expand, strips; };
 
-// us, one side / the other, whole calls: the adapters of a tile dealt to 16 workgroups or not, 777 rows of 24 adapters 26 / 226; shares
-// of K of 8 units or of a thirtieth of it, the same rows 26 / 34; tiles of 16 or 32 rows for the second launch, 4096 rows of
-// prompts 97 / 86; workgroups that walk along the columns (1024 in all) or one for every 256 columns: 64 requests with an adapter of rank 64
-// each 49 / 53, 4096 rows of prompts 86 / 108.
+// Measured, us a call, one side / the other: the adapters of a tile dealt to several workgroups or not, 777 rows of 24 adapters 23 / 226;
+// until there are 256 / 512 / 1024 / 2048 / 4096 workgroups, the same rows 27 / 23 / 24 / 25 / 27, 64 requests with an adapter of rank 64
+// each 56 / 48 / 52 / 48 / 47; shares of K of 8 units or of a thirtieth of it, the 777 rows 26 / 34; tiles of 16 or 32 rows for 4096 rows
+// of prompts 97 / 86; workgroups that walk along the columns (1024 in all) or one for every 256 columns: the 64 requests 49 / 53, 4096
+// rows of prompts 86 / 108.
 static AdapterPlan plan_adapters(const int4mm_adapter_shape& sh) {
     AdapterPlan p;
     const int64_t T = sh.rows, units = sh.in_size / 64;
     auto tiles = [&](int mt) { return (T + 16 * mt - 1) / (16 * mt); };
-    // the most distinct adapters that a tile can hold, and the workgroups that its adapters are dealt to: until there are 2048
+    // the most distinct adapters that a tile can hold, and the workgroups that its adapters are dealt to: until there are 512
     auto distinct = [&](int mt) { return std::min<int64_t>({sh.adapters, T, (16 * mt - 1) / std::min(sh.rows_per_id, T) + 2, 16 * mt}); };
     auto deal = [&](int mt, int64_t workgroups) {
         int d = 1;
-        while (d < distinct(mt) && d < 16 && d * workgroups < 2048) d *= 2;
+        while (d < distinct(mt) && d < 16 && d * workgroups < 512) d *= 2;
         return d;
     };
     p.nt = sh.rank <= 16 ? 1 : sh.rank <= 32 ? 2 : 4;
