@@ -15,9 +15,13 @@
 // (sum x w = s (sum x q - z sum x), the sum of x from a product with ones), which takes 7 instructions a word where rounded weights
 // take 17 and is nearer to the exact product.  The partial sums of the waves meet in LDS.
 //
-// Measured (64 tokens, two of eight experts of 4096 x 11008, int4, us a call): weights rounded, addresses computed, one lane for 16
-// bytes of every row of states 198; exact codes, buffer loads, two units in flight in the order that the waits go by 178; states
-// read row by row and turned in LDS 160.
+// Measured (64 tokens, two of eight experts of 4096 x 11008, int4, us a call on one box): weights rounded, addresses computed, one lane
+// for 16 bytes of every row of states 198; exact codes, buffer loads, two units in flight in the order that the waits go by 178; states
+// read row by row and turned in LDS 172; states straight to LDS, blocks of up to 16 pairs with one row tile 155 - 166.  With all
+// weights from cache 129 before the last step, without the fold of the groups' sums 107: not the bytes, the
+// issue of the fold and the decode and the ends of the workgroups.  Three units in flight are slower (192: registers), so are strips that are
+// neighbours on an XCD (193), and non-temporal loads where the weights fit the last-level cache (37 / 42, 16 experts of 2048 x 1408,
+// 16 pairs each).
 #include "experts.h"
 
 #include <algorithm>
@@ -170,17 +174,12 @@ __device__ __forceinline__ void fill_lut(uint32_t* lut, int t, int threads) {
 
 // ---- a product of up to 16 MT pairs of one expert with 64 columns.  UP: 32 columns of the gate and the same 32 of the other
 // half; the source row of a pair is its token's, the result h.  Else: 64 columns, source and result by place.
-template <int BITS, bool SPARSE, int MT, int WAVES, int DEPTH, bool UP>
-__global__ __launch_bounds__(64 * WAVES, 2) void rows_kernel(ExpertsArgs a) {
+template <int BITS, bool SPARSE, int MT, int WAVES, bool UP>
+__device__ __forceinline__ void rows_tile(const ExpertsArgs& a, const Block& block, char* const (&Xs)[2], uint32_t* lut) {
     using F = RowsFmt<BITS, SPARSE>;
-    constexpr int HEIGHT = 16 * MT;
-    __shared__ __attribute__((aligned(16))) float red[WAVES * HEIGHT * 64];
-    __shared__ __attribute__((aligned(16))) char staged[WAVES * HEIGHT * 128];
-    __shared__ __attribute__((aligned(16))) uint32_t lut[SPARSE ? SPARSE_LUT_WORDS : 4];
+    constexpr int HEIGHT = 16 * MT, DEPTH = 2;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, q = lane >> 4;
-    Block block;
-    if (find_block(a.offsets, a.experts, HEIGHT, blockIdx.x / a.strips, lane, block) >= 0) return;
     const int expert = block.expert, first = block.first, count = block.count;
     const int strip = blockIdx.x % a.strips;
     if constexpr (SPARSE) fill_lut(lut, t, 64 * WAVES);
@@ -196,23 +195,25 @@ __global__ __launch_bounds__(64 * WAVES, 2) void rows_kernel(ExpertsArgs a) {
     const __amdgpu_buffer_rsrc_t z_rsrc = buffer_of(a.zeros + expert * a.scale_stride, groups * (row_bytes / 2));
     const __amdgpu_buffer_rsrc_t x_rsrc = UP ? buffer_of(a.x, a.x_bytes) : buffer_of(a.x + (int64_t)first * a.K, 2u * (uint32_t)count * a.K);
     // states: eight lanes read the 128 bytes of a row (one lane for 16 bytes of every row, as the operands want them, are 64 accesses of
-    // the L1 a load, four times as many), and the wave turns them in LDS of its own: chunk c of row r stands at c ^ (r % 8)
+    // the L1 a load, four times as many), straight to LDS of the wave's own: chunk c of row r stands at c ^ (r % 8)
     uint32_t x_off[2 * MT];
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
         const int at = min(8 * i + (lane >> 3), count - 1);             // (rows beyond the last repeat it and are not written)
-        x_off[i] = 2u * ((uint32_t)(UP ? a.order[first + at] / a.top_k : at) * a.K + 8 * (lane & 7));
+        x_off[i] = 2u * ((uint32_t)(UP ? a.order[first + at] / a.top_k : at) * a.K + 8 * ((lane & 7) ^ (lane >> 3)));
     }
-    // (written and read as the same type: without a barrier between, the compiler has to see that they are the same memory)
-    char* const stage = staged + wave * (HEIGHT * 128);
-    char* const stage_to = stage + (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16;
     const uint32_t w_off = 4u * col + packed_row<BITS, SPARSE>(q) * row_bytes, w_off2 = 4u * col + packed_row2<BITS, SPARSE>(q) * row_bytes;
 
     struct Unit {                                     // 64 k
         u32x4 w[2][F::LOADS];
         u32x2 s, z;
     };
-    auto load = [&](Unit& u, int unit) __attribute__((always_inline)) {
+    constexpr int UNIT_LOADS = 2 * MT + 2 * F::LOADS + 2;
+    auto load = [&](Unit& u, char* stage, int unit) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < 2 * MT; ++c)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(x_rsrc, (__attribute__((address_space(3))) void*)(stage + wave * (HEIGHT * 128) + c * 1024), 16,
+                                                     x_off[c], 128u * unit, 0, 0);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const uint32_t blk = (uint32_t)(2 * unit + b) * row_bytes;
@@ -240,13 +241,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void rows_kernel(ExpertsArgs a) {
     clear_group();
     clear(sum);
     const h16x8 ones = bitcast<h16x8>(u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
-    auto multiply = [&](auto mode, const Unit& u) __attribute__((always_inline)) {
+    auto multiply = [&](auto mode, const Unit& u, const char* stage) __attribute__((always_inline)) {
         h16x8 x[2][MT];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                x[b][m] = bitcast<h16x8>(*reinterpret_cast<const u32x4*>(stage + (16 * m + n) * 128 + (((4 * b + q) ^ n) & 7) * 16));
+                x[b][m] = bitcast<h16x8>(*reinterpret_cast<const u32x4*>(stage + (wave * HEIGHT + 16 * m + n) * 128 + (((4 * b + q) ^ n) & 7) * 16));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             Values<BITS, SPARSE, decltype(mode)::value> co;
@@ -289,15 +290,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void rows_kernel(ExpertsArgs a) {
     if (u0 < u1) {
         int left = a.group_units - (u0 - magic_div(u0, a.group_units, a.group_magic) * a.group_units);
         Unit ring[DEPTH];
-        u32x4 x[2 * MT];                              // the next unit's: they come from the L2
-        auto load_x = [&](int unit) __attribute__((always_inline)) {
-#pragma unroll
-            for (int c = 0; c < 2 * MT; ++c) x[c] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, x_off[c], 128u * unit, 0);
-        };
-        load_x(u0);
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-            load(ring[d], min(u0 + d, u1 - 1));
+            load(ring[d], Xs[d], min(u0 + d, u1 - 1));
             __builtin_amdgcn_sched_barrier(0);        // (in this order, which the waits in the loop go by)
         }
 #pragma unroll 1
@@ -305,33 +300,39 @@ __global__ __launch_bounds__(64 * WAVES, 2) void rows_kernel(ExpertsArgs a) {
 #pragma unroll
             for (int d = 0; d < DEPTH; ++d) {
                 const Unit& now = ring[d];
-#pragma unroll
-                for (int c = 0; c < 2 * MT; ++c) *reinterpret_cast<u32x4*>(stage_to + c * 1024) = x[c];
-                load_x(min(i + d + 1, u1 - 1));
+                // all loads but those of the younger units have arrived
+                __builtin_amdgcn_s_waitcnt(wait_counts((DEPTH - 1) * UNIT_LOADS, 15));
                 __builtin_amdgcn_sched_barrier(0);
                 if (i + d < u1) {
-                    if (any_negative(now.s[0], now.s[1])) multiply(std::true_type{}, now);
-                    else multiply(std::false_type{}, now);
+                    if (any_negative(now.s[0], now.s[1])) multiply(std::true_type{}, now, Xs[d]);
+                    else multiply(std::false_type{}, now, Xs[d]);
                     if (--left == 0 || i + d == u1 - 1) {
                         fold(now);
                         left = a.group_units;
                     }
                 }
-                load(ring[d], min(i + d + DEPTH, u1 - 1));
+                __builtin_amdgcn_sched_barrier(0);
+                load(ring[d], Xs[d], min(i + d + DEPTH, u1 - 1));
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
+    // (no load to LDS is in flight any more)
+    __builtin_amdgcn_s_waitcnt(wait_counts(0, 15));
+    __syncthreads();
     // register r of tile (m, j): row 16 m + 4 q + r, column 4 n + j of the strip
+    float* const red[2] = {reinterpret_cast<float*>(Xs[0]), reinterpret_cast<float*>(Xs[1])};
+    float* const to = (wave < WAVES / 2 ? red[0] : red[1]) + wave % (WAVES / 2) * (HEIGHT * 64);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            *reinterpret_cast<f32x4*>(red + (wave * HEIGHT + 16 * m + 4 * q + r) * 64 + 4 * n) = f32x4{sum[m][0][r], sum[m][1][r], sum[m][2][r], sum[m][3][r]};
+            *reinterpret_cast<f32x4*>(to + (16 * m + 4 * q + r) * 64 + 4 * n) = f32x4{sum[m][0][r], sum[m][1][r], sum[m][2][r], sum[m][3][r]};
     __syncthreads();
     auto total = [&](int row, int c) __attribute__((always_inline)) {
-        f32x4 s = *reinterpret_cast<const f32x4*>(red + row * 64 + c);
-        for (int w = 1; w < WAVES; ++w) s += *reinterpret_cast<const f32x4*>(red + (w * HEIGHT + row) * 64 + c);
+        f32x4 s = *reinterpret_cast<const f32x4*>(red[0] + row * 64 + c);
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) s += *reinterpret_cast<const f32x4*>(red[w / (WAVES / 2)] + (w % (WAVES / 2) * HEIGHT + row) * 64 + c);
         return s;
     };
     constexpr int QUADS = UP ? 8 : 16;                // quadruples of results in a row
@@ -348,6 +349,20 @@ __global__ __launch_bounds__(64 * WAVES, 2) void rows_kernel(ExpertsArgs a) {
             *reinterpret_cast<f32x4*>(a.part + (int64_t)(first + row) * a.S + 64 * strip + c) = total(row, c);
         }
     }
+}
+
+template <int BITS, bool SPARSE, int MT, int WAVES, bool UP>
+__global__ __launch_bounds__(64 * WAVES, 2) void rows_kernel(ExpertsArgs a) {
+    constexpr int STAGE = WAVES * 16 * MT * 128;
+    // the states of the two units in flight (arrays of their own, so that the compiler sees which loads a read has to wait for); behind
+    // the loop the waves' partial sums
+    __shared__ __attribute__((aligned(16))) char X0[STAGE], X1[STAGE];
+    __shared__ __attribute__((aligned(16))) uint32_t lut[SPARSE ? SPARSE_LUT_WORDS : 4];
+    char* const Xs[2] = {X0, X1};
+    Block block;
+    if (find_block(a.offsets, a.experts, 16 * MT, blockIdx.x / a.strips, threadIdx.x & 63, block) >= 0) return;
+    if (MT == 2 && block.count <= 16) rows_tile<BITS, SPARSE, 1, WAVES, UP>(a, block, Xs, lut);
+    else rows_tile<BITS, SPARSE, MT, WAVES, UP>(a, block, Xs, lut);
 }
 
 // ---- few pairs, hardly two of them of the same expert: no order, a workgroup takes a pair and 64 columns, two launches in all.
@@ -562,10 +577,10 @@ static void launch_rows(ExpertsArgs a, int height, int64_t pairs, hipStream_t st
     const dim3 grid((unsigned)(std::min<int64_t>(pairs, a.experts + pairs / height) * a.strips));
     if constexpr (low_blocks(BITS, SPARSE))
         if (height == 16) {
-            hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 1, 8, 2, UP>), grid, dim3(512), 0, st, a);
+            hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 1, 8, UP>), grid, dim3(512), 0, st, a);
             return;
         }
-    hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 2, 4, 2, UP>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 2, 4, UP>), grid, dim3(256), 0, st, a);
 }
 
 template <bool UP>
