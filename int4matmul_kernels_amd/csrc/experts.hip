@@ -172,12 +172,13 @@ __device__ __forceinline__ void fill_lut(uint32_t* lut, int t, int threads) {
     __syncthreads();
 }
 
-// ---- a product of up to 16 MT pairs of one expert with 64 columns.  UP: 32 columns of the gate and the same 32 of the other
+// ---- a product of up to 32 pairs of one expert with 64 columns, 16 MT of them in a tile's rows.  UP: 32 columns of the gate and the same 32 of the other
 // half; the source row of a pair is its token's, the result h.  Else: 64 columns, source and result by place.
-template <int BITS, bool SPARSE, int MT, int WAVES, bool UP>
+constexpr int ROWS_HEIGHT = 32, ROWS_WAVES = 4;
+template <int BITS, bool SPARSE, int MT, bool UP>
 __device__ __forceinline__ void rows_tile(const ExpertsArgs& a, const Block& block, char* const (&Xs)[2], uint32_t* lut) {
     using F = RowsFmt<BITS, SPARSE>;
-    constexpr int HEIGHT = 16 * MT, DEPTH = 2;
+    constexpr int HEIGHT = 16 * MT, WAVES = ROWS_WAVES, DEPTH = 2;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, q = lane >> 4;
     const int expert = block.expert, first = block.first, count = block.count;
@@ -351,18 +352,18 @@ __device__ __forceinline__ void rows_tile(const ExpertsArgs& a, const Block& blo
     }
 }
 
-template <int BITS, bool SPARSE, int MT, int WAVES, bool UP>
-__global__ __launch_bounds__(64 * WAVES, 2) void rows_kernel(ExpertsArgs a) {
-    constexpr int STAGE = WAVES * 16 * MT * 128;
+template <int BITS, bool SPARSE, bool UP>
+__global__ __launch_bounds__(64 * ROWS_WAVES, 2) void rows_kernel(ExpertsArgs a) {
+    constexpr int STAGE = ROWS_WAVES * ROWS_HEIGHT * 128;
     // the states of the two units in flight (arrays of their own, so that the compiler sees which loads a read has to wait for); behind
     // the loop the waves' partial sums
     __shared__ __attribute__((aligned(16))) char X0[STAGE], X1[STAGE];
     __shared__ __attribute__((aligned(16))) uint32_t lut[SPARSE ? SPARSE_LUT_WORDS : 4];
     char* const Xs[2] = {X0, X1};
     Block block;
-    if (find_block(a.offsets, a.experts, 16 * MT, blockIdx.x / a.strips, threadIdx.x & 63, block) >= 0) return;
-    if (MT == 2 && block.count <= 16) rows_tile<BITS, SPARSE, 1, WAVES, UP>(a, block, Xs, lut);
-    else rows_tile<BITS, SPARSE, MT, WAVES, UP>(a, block, Xs, lut);
+    if (find_block(a.offsets, a.experts, ROWS_HEIGHT, blockIdx.x / a.strips, threadIdx.x & 63, block) >= 0) return;
+    if (block.count <= 16) rows_tile<BITS, SPARSE, 1, UP>(a, block, Xs, lut);
+    else rows_tile<BITS, SPARSE, 2, UP>(a, block, Xs, lut);
 }
 
 // ---- few pairs, hardly two of them of the same expert: no order, a workgroup takes a pair and 64 columns, two launches in all.
@@ -537,22 +538,19 @@ __global__ __launch_bounds__(256) void combine_kernel(h16* outs, const T* part, 
 //
 // A pair by itself: one token, or so few pairs that hardly two of them share an expert.
 //
-// Blocks of rows_kernel up to a mean of 40, then tiles.  us a call, 16 experts of 2048 x 1408, means of 8 / 32 / 48 / 64: blocks of
-// 32 pairs int4 36 / 50 / 60 / 70, int3 41 / 58 / 68 / 79, 16:32 47 / 66 / 78 / 92; tiles of 64 (and at 64: 96) rows int4 - / 56 / 56 / 58,
-// int3 - / 58 / 59 / 61, 16:32 - / 79 / 78 / 82.  Blocks of 64 pairs were slower than either everywhere.  Blocks of 16 pairs, of eight
-// waves: int4 at means of 4 / 8 / 12 30 / 34 / 36 where 32 take 36 / 36 / 36, but int3 40 / 45 / 51 and 41 / 41 / 41, 16:32 47 / 53 / 60 and
-// 48 / 47 / 46.
+// Blocks of rows_kernel up to a mean of 40, then tiles.  us a call, 16 experts of 2048 x 1408, means of 32 / 48 / 64 / 96: blocks int4 43 /
+// 54 / 63 / 84, int3 49 / 62 / 72 / 97, int2 46 / 58 / 67 / 90, 16:32 60 / 72 / 86 / 116; tiles int4 - / 53 / 56 / 63, int3 - / 58 / 60 / 65, int2 - /
+// 52 / 55 / 59, 16:32 - / 77 / 79 / 85.
 //
 // The height of the tiles: rounds of 256 workgroups times what a K step takes, with the blocks that an expert is expected to need
 // (normal around the mean; the last step's length from the tile kernels' cost model, matmul.hip).  int4, means of 64 / 96 / 128 / 192 /
 // 256 / 384, 64 rows 81 / 83 / 102 / 132 / 179 / 228, 96: 58 / 76 / 91 / 113 / 146 / 205, 128: 62 / 65 / 98 / 104 / 128 / 170, 192: 70 / 73 / 77 /
 // 120 / 126 / 161, 256: 78 / 81 / 85 / 94 / 141 / 154.
-constexpr bool low_blocks(int bits, bool sparse) { return bits != 3 && !sparse; }
-struct ExpertsPlan { bool single; int height; int tm; };         // tm: 0 (rows_kernel with blocks of `height` pairs) or tiles of 32 tm rows
-static ExpertsPlan plan_experts(int bits, bool sparse, const int4mm_experts_shape& sh) {
+struct ExpertsPlan { bool single; int tm; };         // tm: 0 (rows_kernel) or tiles of 32 tm rows
+static ExpertsPlan plan_experts(const int4mm_experts_shape& sh) {
     const int64_t pairs = sh.tokens * sh.top_k;
     const double mean = (double)pairs / sh.experts;
-    ExpertsPlan p{pairs <= 64 && (sh.tokens == 1 || 2 * pairs <= sh.experts), low_blocks(bits, sparse) && mean <= 8 ? 16 : 32, 0};
+    ExpertsPlan p{pairs <= 64 && (sh.tokens == 1 || 2 * pairs <= sh.experts), 0};
     if (p.single || mean <= 40) return p;
     const double step[] = {0.30, 0.335, 0.373, 0.466, 0.555}, strips = (double)((sh.width + 127) / 128);
     const int tms[] = {2, 3, 4, 6, 8};
@@ -571,24 +569,14 @@ static ExpertsPlan plan_experts(int bits, bool sparse, const int4mm_experts_shap
     return p;
 }
 
-template <int BITS, bool SPARSE, bool UP>
-static void launch_rows(ExpertsArgs a, int height, int64_t pairs, hipStream_t st) {
-    a.strips = a.S / 64;
-    const dim3 grid((unsigned)(std::min<int64_t>(pairs, a.experts + pairs / height) * a.strips));
-    if constexpr (low_blocks(BITS, SPARSE))
-        if (height == 16) {
-            hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 1, 8, UP>), grid, dim3(512), 0, st, a);
-            return;
-        }
-    hipLaunchKernelGGL((rows_kernel<BITS, SPARSE, 2, 4, UP>), grid, dim3(256), 0, st, a);
-}
-
 template <bool UP>
-static void rows_product(int bits, const ExpertsArgs& a, int height, int64_t pairs, hipStream_t st) {
-    if (a.mask) launch_rows<4, true, UP>(a, height, pairs, st);
-    else if (bits == 4) launch_rows<4, false, UP>(a, height, pairs, st);
-    else if (bits == 3) launch_rows<3, false, UP>(a, height, pairs, st);
-    else launch_rows<2, false, UP>(a, height, pairs, st);
+static void rows_product(int bits, ExpertsArgs a, int64_t pairs, hipStream_t st) {
+    a.strips = a.S / 64;
+    const dim3 grid((unsigned)(std::min<int64_t>(pairs, a.experts + pairs / ROWS_HEIGHT) * a.strips)), block(64 * ROWS_WAVES);
+    if (a.mask) hipLaunchKernelGGL((rows_kernel<4, true, UP>), grid, block, 0, st, a);
+    else if (bits == 4) hipLaunchKernelGGL((rows_kernel<4, false, UP>), grid, block, 0, st, a);
+    else if (bits == 3) hipLaunchKernelGGL((rows_kernel<3, false, UP>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((rows_kernel<2, false, UP>), grid, block, 0, st, a);
 }
 
 template <bool UP>
@@ -621,7 +609,7 @@ static int check_experts(int bits, const int4mm_experts_shape* sh, bool sparse) 
     // (a matrix, and the rows of a block, are addressed with 31 bits)
     if (K >= limit / 128 || F >= limit / 128 || K * F >= limit) return INT4MM_ERR_SHAPE;
     if (sh->top_k > 1024 || sh->tokens >= limit) return INT4MM_ERR_SHAPE;
-    // (a grid of one dimension has a workgroup for every 16 pairs, or expert, and 64 columns)
+    // (a grid of one dimension has a workgroup for every 32 pairs, or expert, and 64 columns)
     if ((tokens_at_once(*sh) * sh->top_k / 16 + sh->experts) * (std::max(K, 2 * F) / 64) >= limit) return INT4MM_ERR_SHAPE;
     return INT4MM_OK;
 }
@@ -662,7 +650,7 @@ static int experts_share(int bits, bool sparse, h16* outs, const h16* x, const f
     a.ids = ids;
     a.weights = weights;
     a.outs = outs;
-    const ExpertsPlan plan = plan_experts(bits, sparse, *sh);
+    const ExpertsPlan plan = plan_experts(*sh);
     if (!plan.single)
         hipLaunchKernelGGL(plan_kernel, dim3(E), dim3(1024), 0, st, a.ids, const_cast<int*>(a.offsets), const_cast<int*>(a.order), place, (int)pairs, E);
     if (const int rc = check_launch("experts_forward")) return rc;
@@ -680,7 +668,7 @@ static int experts_share(int bits, bool sparse, h16* outs, const h16* x, const f
     a.x_bytes = (uint32_t)(sh->tokens * K * 2);
     if (plan.single) token_product<true>(bits, a, pairs, st);
     else if (plan.tm) launch_experts_tiles(bits, a, plan.tm, pairs, true, st);
-    else rows_product<true>(bits, a, plan.height, pairs, st);
+    else rows_product<true>(bits, a, pairs, st);
     if (const int rc = check_launch("experts_forward")) return rc;
     a.x = a.h;
     a.matrix = static_cast<const uint32_t*>(down_matrix);
@@ -700,7 +688,7 @@ static int experts_share(int bits, bool sparse, h16* outs, const h16* x, const f
         a.h = reinterpret_cast<h16*>(ws + parts.part);
         launch_experts_tiles(bits, a, plan.tm, pairs, false, st);
     } else {
-        rows_product<false>(bits, a, plan.height, pairs, st);
+        rows_product<false>(bits, a, pairs, st);
     }
     if (const int rc = check_launch("experts_forward")) return rc;
     const int columns = (int)((K + (plan.tm ? 2047 : 1023)) / (plan.tm ? 2048 : 1024));
