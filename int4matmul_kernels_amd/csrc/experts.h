@@ -1,4 +1,4 @@
-// What the experts' kernels share: their arguments, and which expert's pairs a block of a grid takes.
+// What the experts' kernels share: their arguments, and which expert's pairs (or adapter's rows) a block of a grid takes.
 #pragma once
 
 #include "pipe.h"
@@ -55,6 +55,9 @@ __device__ __forceinline__ int find_block(const int* offsets, int experts, int h
     }
     return before;
 }
+
+// experts.hip: rows in the order of their ids, stable, an id outside 0 ... buckets - 2 in the last bucket; offsets [buckets + 1]
+void launch_rows_by_id(const int* ids, int* offsets, int* order, int rows, int buckets, hipStream_t st);
 
 // experts_tiles.hip: both products in tiles of 32 tm rows (tm: 2, 3, 4, 6 or 8) and 256 columns
 void launch_experts_tiles(int bits, const ExpertsArgs& a, int tm, int64_t pairs, bool gated, hipStream_t st);

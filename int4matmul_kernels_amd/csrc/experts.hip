@@ -38,7 +38,9 @@ template <> struct RowsFmt<4, true> { static constexpr int ROWS = 2, LOADS = 3; 
 // ---- pairs in the order of their experts: workgroup e finds how many pairs belong to lower experts, and places its own.  Each
 // of the 16 waves takes a share of the pairs, twice: counting, then placing; no atomics, the order is that of the pairs.
 // A wave reads 256 pairs at a time, four neighbours a lane, and keeps the first 2048 of its share in registers: one trip to memory.
+// REST: an id outside belongs to the last expert, and no places are asked for.
 struct __attribute__((packed, aligned(4))) FourIds { int v[4]; };
+template <bool REST>
 __global__ __launch_bounds__(1024) void plan_kernel(const int* ids, int* offsets, int* order, int* place, int pairs, int experts) {
     constexpr int DEPTH = 8;
     __shared__ int of_wave[16], lower_of_wave[16];
@@ -54,6 +56,11 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int* ids, int* offsets
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = p + j < to ? ids[p + j] : -1;
+        }
+        if constexpr (REST) {
+            // (below 0: not a pair)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = p + j >= to ? -1 : (uint32_t)v[j] < (uint32_t)experts ? v[j] : experts - 1;
         }
     };
     int mine = 0, below = 0;
@@ -108,8 +115,9 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int* ids, int* offsets
             const int p = i + 4 * lane + j;
             if (v[j] == e) {
                 order[where] = p;
-                place[p] = where++;
-            } else if (e == 0 && p < to && (uint32_t)v[j] >= (uint32_t)experts) {
+                if constexpr (!REST) place[p] = where;
+                ++where;
+            } else if (!REST && e == 0 && p < to && (uint32_t)v[j] >= (uint32_t)experts) {
                 place[p] = -1;
             }
         }
@@ -122,6 +130,10 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int* ids, int* offsets
         load(v, i);
         put(v, i);
     }
+}
+
+void launch_rows_by_id(const int* ids, int* offsets, int* order, int rows, int buckets, hipStream_t st) {
+    hipLaunchKernelGGL(plan_kernel<true>, dim3(buckets), dim3(1024), 0, st, ids, offsets, order, (int*)nullptr, rows, buckets);
 }
 
 // The operand of a lane, 8 k of one column, from the words that it has loaded of a 32-row block: `lo` its packed word (int3: and the
@@ -652,7 +664,7 @@ static int experts_share(int bits, bool sparse, h16* outs, const h16* x, const f
     a.outs = outs;
     const ExpertsPlan plan = plan_experts(*sh);
     if (!plan.single)
-        hipLaunchKernelGGL(plan_kernel, dim3(E), dim3(1024), 0, st, a.ids, const_cast<int*>(a.offsets), const_cast<int*>(a.order), place, (int)pairs, E);
+        hipLaunchKernelGGL(plan_kernel<false>, dim3(E), dim3(1024), 0, st, a.ids, const_cast<int*>(a.offsets), const_cast<int*>(a.order), place, (int)pairs, E);
     if (const int rc = check_launch("experts_forward")) return rc;
     auto rows_of = [&](int64_t k) { return sparse ? k / 16 : k * bits / 32; };
     a.x = x;

@@ -253,3 +253,56 @@ def test_refusals(ext):
         add(ext, problem((2, 1), 2, 8, 96, 64))
     with pytest.raises(RuntimeError, match="no backward"):
         add(ext, p, x=p["x"].clone().requires_grad_())
+
+
+@pytest.mark.parametrize("rank", [5, 40, 130])
+@pytest.mark.parametrize("T,n", [(300, 3), (1100, 30), (2500, 70), (4000, 250)])
+def test_many_rows_with_ids_of_their_own(ext, T, n, rank):
+    """random ids, one adapter for all rows but one, adapters without a row, no adapter at all; in place too"""
+    p = problem((1, T), n, rank, 128, 192, per_row=True, seed=T)
+    one = torch.full_like(p["ids"], n - 1)
+    one[0, T // 2] = 0
+    outside = torch.tensor([-1, n, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device="cuda").repeat(T)[:T].reshape(1, T)
+    mixed = torch.where(torch.arange(T, device="cuda") % 3 == 0, outside, p["ids"] // 2)
+    for ids in (p["ids"], one, mixed.to(torch.int32).contiguous()):
+        q = dict(p, ids=ids)
+        got = add(ext, q)
+        close(got, dict(q, ids=torch.where((ids < 0) | (ids >= n), -1, ids)))
+        base = p["base"].clone()
+        ext.low_rank_add(base, p["x"], p["down"], p["up"], p["scales"], ids, base)
+        assert torch.equal(base, got)
+    assert torch.equal(add(ext, p, ids=outside), p["base"])
+
+
+def test_many_rows_with_ids_of_their_own_captured(ext):
+    a, b = problem((900, 1), 12, 16, seed=1), problem((900, 1), 12, 16, seed=2)
+    b.update({n: a[n] for n in ("down", "up", "scales")})
+    held = {n: a[n].clone() for n in ("base", "x", "ids")}
+    want = {id(q): add(ext, q) for q in (a, b)}
+    close(want[id(a)], a)
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            outs.append(add(ext, a, **held))
+    for q in (a, b, a, b):
+        for n in held:
+            held[n].copy_(q[n])
+        for g in graphs:
+            g.replay()
+        eager = add(ext, q)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[id(q)]) and all(torch.equal(o, eager) for o in outs)
+
+
+def test_rows_in_order_leave_what_lies_behind(ext):
+    from int4matmul_kernels_amd import capi
+    p = problem((500, 1), 9, 20, seed=7)
+    outs = torch.full((520, 192), 7.0, dtype=torch.float16, device="cuda")
+    ws = capi.new_adapters_workspace(500, 1, p["down"], p["up"])
+    ws.fill_(255)
+    capi.low_rank_add(outs[:500], p["base"][:, 0], p["x"][:, 0], p["down"], p["up"], p["scales"], p["ids"], 1, ws)
+    assert torch.equal(outs[:500], add(ext, p)[:, 0]) and torch.all(outs[500:] == 7)
+    with pytest.raises(capi.Int4mmError) as e:
+        capi.low_rank_add(outs[:500], p["base"][:, 0], p["x"][:, 0], p["down"], p["up"], p["scales"], p["ids"], 1, ws[:-16])
+    assert e.value.code == 6
