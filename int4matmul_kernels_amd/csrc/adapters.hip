@@ -405,9 +405,11 @@ static AdapterPlan plan_adapters(const int4mm_adapter_shape& sh) {
         return d;
     };
     p.deal_shrink = deal(p.tiles * rank_parts);
-    // (a share is at least the two units that a wave takes at once, and there are at most 16 to add up)
+    // (a share is at least the two units that a wave takes at once, and there are at most 16 to add up, fewer where the tiles are many:
+    // every workgroup of expand_kernel adds them up.  Up to 1024 / 8192 workgroups, prompts of 256 rows, 16 adapters of rank 64, 8192 x 8192,
+    // 74 / 94; 4096 rows of one of rank 128, 4096 x 11008, 134 / 152)
     const int64_t workgroups = p.tiles * rank_parts * p.deal_shrink;
-    p.units_per_split = (int)std::max<int64_t>({8, (units + 15) / 16, (units * workgroups + 8191) / 8192});
+    p.units_per_split = (int)std::max<int64_t>({8, (units + 15) / 16, (units * workgroups + 1023) / 1024});
     p.ksplit = (int)((units + p.units_per_split - 1) / p.units_per_split);
     const int64_t strips = (sh.out_size + 255) / 256;
     p.deal_expand = deal(p.tiles * strips);

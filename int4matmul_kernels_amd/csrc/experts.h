@@ -22,6 +22,7 @@ struct ExpertsArgs {
     int64_t matrix_stride, mask_stride, scale_stride;   // elements from an expert to the next
     int experts, top_k, K, S;      // S: columns of the matrix (up: 2 F)
     int group_units, strips;       // strips: of columns
+    int height;                    // of the tiles
     uint32_t group_magic;
     uint32_t x_bytes;              // up: of all source rows
 };
@@ -59,7 +60,7 @@ __device__ __forceinline__ int find_block(const int* offsets, int experts, int h
 // experts.hip: rows in the order of their ids, stable, an id outside 0 ... buckets - 2 in the last bucket; offsets [buckets + 1]
 void launch_rows_by_id(const int* ids, int* offsets, int* order, int rows, int buckets, hipStream_t st);
 
-// experts_tiles.hip: both products in tiles of 32 tm rows (tm: 2, 3, 4, 6 or 8) and 256 columns
-void launch_experts_tiles(int bits, const ExpertsArgs& a, int tm, int64_t pairs, bool gated, hipStream_t st);
+// experts_tiles.hip: both products in tiles of up to `height` (64, 128, 192 or 256) rows and 256 columns
+void launch_experts_tiles(int bits, ExpertsArgs a, int height, int64_t pairs, bool gated, hipStream_t st);
 
 }  // namespace i4

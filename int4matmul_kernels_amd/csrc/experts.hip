@@ -554,30 +554,37 @@ __global__ __launch_bounds__(256) void combine_kernel(h16* outs, const T* part, 
 // 54 / 63 / 84, int3 49 / 62 / 72 / 97, int2 46 / 58 / 67 / 90, 16:32 60 / 72 / 86 / 116; tiles int4 - / 53 / 56 / 63, int3 - / 58 / 60 / 65, int2 - /
 // 52 / 55 / 59, 16:32 - / 77 / 79 / 85.
 //
-// The height of the tiles: rounds of 256 workgroups times what a K step takes, with the blocks that an expert is expected to need
-// (normal around the mean; the last step's length from the tile kernels' cost model, matmul.hip).  int4, means of 64 / 96 / 128 / 192 /
-// 256 / 384, 64 rows 81 / 83 / 102 / 132 / 179 / 228, 96: 58 / 76 / 91 / 113 / 146 / 205, 128: 62 / 65 / 98 / 104 / 128 / 170, 192: 70 / 73 / 77 /
-// 120 / 126 / 161, 256: 78 / 81 / 85 / 94 / 141 / 154.
-struct ExpertsPlan { bool single; int tm; };         // tm: 0 (rows_kernel) or tiles of 32 tm rows
-static ExpertsPlan plan_experts(const int4mm_experts_shape& sh) {
-    const int64_t pairs = sh.tokens * sh.top_k;
-    const double mean = (double)pairs / sh.experts;
-    ExpertsPlan p{pairs <= 64 && (sh.tokens == 1 || 2 * pairs <= sh.experts), 0};
-    if (p.single || mean <= 40) return p;
-    const double step[] = {0.30, 0.335, 0.373, 0.466, 0.555}, strips = (double)((sh.width + 127) / 128);
-    const int tms[] = {2, 3, 4, 6, 8};
-    double best = 1e30;
-    for (int i = 0; i < 5; ++i) {
-        const int h = 32 * tms[i];
-        // E ceil(c / h) = 1 + sum over n >= 1 of P(c > n h), which is 1 for the first of them
-        const double deviation = std::sqrt(mean);
-        int64_t n = std::max<int64_t>(1, (int64_t)((mean - 4 * deviation) / h));
-        double blocks = (double)n;
-        for (; n * h < mean + 4 * deviation; ++n) blocks += 0.5 * std::erfc((n * h - mean) / (deviation * 1.41421356));
-        const double rounds = sh.experts * blocks * strips / 256.0;
-        const double us = (rounds < 8 ? std::ceil(rounds) : rounds + 0.5) * step[i];
-        if (us < best) best = us, p.tm = tms[i];
+// The height of the tiles, for each product: a tile of up to 64 / 128 / 192 / 256 rows takes 8 us and, on a full grid, 0.43 / 0.53 / 0.69 / 0.86 a
+// K step; the tiles are those of experts that are asked unevenly, with a deviation of half the mean beside that of independent choices.
+struct ExpertsPlan { bool single, tiles; int up, down; };          // up, down: heights of the tiles
+static double tiles_us(double mean, int experts, int height, int64_t strips, int64_t steps) {
+    // (the middles of eight equal parts of the normal distribution)
+    const double parts[] = {-1.534, -0.887, -0.489, -0.157, 0.157, 0.489, 0.887, 1.534}, step[] = {0, 0.43, 0.53, 0.69, 0.86};
+    const double deviation = std::sqrt(mean + 0.25 * mean * mean);
+    double us = 0, tiles = 0, longest = 0;
+    for (double z : parts) {
+        const int rows = std::max(1, (int)(mean + deviation * z)), full = rows / height, rest = rows % height;
+        const double whole = 8.0 + steps * step[height / 64], last = rest ? 8.0 + steps * step[(rest + 63) / 64] : 0.0;
+        us += full * whole + last;
+        tiles += full + (rest > 0);
+        longest = std::max(longest, full ? whole : last);
     }
+    const double each = us / tiles, rounds = tiles / 8 * experts * strips / 256.0;
+    return rounds <= 1 ? longest : rounds * each + 0.7 * longest;
+}
+static ExpertsPlan plan_experts(const int4mm_experts_shape& sh) {
+    const int64_t pairs = sh.tokens * sh.top_k, K = sh.in_size, F = sh.width;
+    const double mean = (double)pairs / sh.experts;
+    ExpertsPlan p{pairs <= 64 && (sh.tokens == 1 || 2 * pairs <= sh.experts), mean > 40, 128, 128};
+    if (p.single || !p.tiles) return p;
+    auto height = [&](int64_t strips, int64_t steps) {
+        int best = 64;
+        for (int h = 128; h <= 256; h += 64)
+            if (tiles_us(mean, (int)sh.experts, h, strips, steps) < tiles_us(mean, (int)sh.experts, best, strips, steps)) best = h;
+        return best;
+    };
+    p.up = height((F + 127) / 128, K / 32);
+    p.down = height((K + 255) / 256, F / 32);
     return p;
 }
 
@@ -679,7 +686,7 @@ static int experts_share(int bits, bool sparse, h16* outs, const h16* x, const f
     a.scale_stride = sh->up_groups * 2 * F;
     a.x_bytes = (uint32_t)(sh->tokens * K * 2);
     if (plan.single) token_product<true>(bits, a, pairs, st);
-    else if (plan.tm) launch_experts_tiles(bits, a, plan.tm, pairs, true, st);
+    else if (plan.tiles) launch_experts_tiles(bits, a, plan.up, pairs, true, st);
     else rows_product<true>(bits, a, pairs, st);
     if (const int rc = check_launch("experts_forward")) return rc;
     a.x = a.h;
@@ -696,16 +703,16 @@ static int experts_share(int bits, bool sparse, h16* outs, const h16* x, const f
         token_product<false>(bits, a, pairs, st);
         return check_launch("experts_forward");
     }
-    if (plan.tm) {
+    if (plan.tiles) {
         a.h = reinterpret_cast<h16*>(ws + parts.part);
-        launch_experts_tiles(bits, a, plan.tm, pairs, false, st);
+        launch_experts_tiles(bits, a, plan.down, pairs, false, st);
     } else {
         rows_product<false>(bits, a, pairs, st);
     }
     if (const int rc = check_launch("experts_forward")) return rc;
-    const int columns = (int)((K + (plan.tm ? 2047 : 1023)) / (plan.tm ? 2048 : 1024));
+    const int columns = (int)((K + (plan.tiles ? 2047 : 1023)) / (plan.tiles ? 2048 : 1024));
     const dim3 grid((unsigned)(sh->tokens * columns));
-    if (plan.tm)
+    if (plan.tiles)
         hipLaunchKernelGGL(combine_kernel<h16>, grid, dim3(256), 0, st, a.outs, a.h, a.weights, place,
                            a.top_k, (int)K, columns);
     else
