@@ -60,7 +60,7 @@ __device__ __forceinline__ int find_block(const int* offsets, int experts, int h
 // experts.hip: rows in the order of their ids, stable, an id outside 0 ... buckets - 2 in the last bucket; offsets [buckets + 1]
 void launch_rows_by_id(const int* ids, int* offsets, int* order, int rows, int buckets, hipStream_t st);
 
-// experts_tiles.hip: both products in tiles of up to `height` (64, 128, 192 or 256) rows and 256 columns
+// experts_tiles.hip: both products in tiles of up to `height` (64, 96, 128, 192 or 256) rows and 256 columns
 void launch_experts_tiles(int bits, ExpertsArgs a, int height, int64_t pairs, bool gated, hipStream_t st);
 
 }  // namespace i4

@@ -554,23 +554,24 @@ __global__ __launch_bounds__(256) void combine_kernel(h16* outs, const T* part, 
 // 54 / 63 / 84, int3 49 / 62 / 72 / 97, int2 46 / 58 / 67 / 90, 16:32 60 / 72 / 86 / 116; tiles int4 - / 53 / 56 / 63, int3 - / 58 / 60 / 65, int2 - /
 // 52 / 55 / 59, 16:32 - / 77 / 79 / 85.
 //
-// The height of the tiles, for each product: a tile of up to 64 / 128 / 192 / 256 rows takes 8 us and, on a full grid, 0.43 / 0.53 / 0.69 / 0.86 a
-// K step; the tiles are those of experts that are asked unevenly, with a deviation of half the mean beside that of independent choices.
+// The height of the tiles, for each product: a tile of up to 64 / 96 / 128 / 192 / 256 rows takes 8 us and, on a full grid, 0.43 / 0.47 / 0.53 / 0.69 /
+// 0.86 a K step; the tiles are those of experts that are asked unevenly, with a deviation of half the mean beside that of independent choices.
 struct ExpertsPlan { bool single, tiles; int up, down; };          // up, down: heights of the tiles
 static double tiles_us(double mean, int experts, int height, int64_t strips, int64_t steps) {
     // (the middles of eight equal parts of the normal distribution)
-    const double parts[] = {-1.534, -0.887, -0.489, -0.157, 0.157, 0.489, 0.887, 1.534}, step[] = {0, 0.43, 0.53, 0.69, 0.86};
+    const double parts[] = {-1.534, -0.887, -0.489, -0.157, 0.157, 0.489, 0.887, 1.534}, step[] = {0.43, 0.43, 0.47, 0.53, 0.69, 0.69, 0.86, 0.86};
     const double deviation = std::sqrt(mean + 0.25 * mean * mean);
     double us = 0, tiles = 0, longest = 0;
     for (double z : parts) {
         const int rows = std::max(1, (int)(mean + deviation * z)), full = rows / height, rest = rows % height;
-        const double whole = 8.0 + steps * step[height / 64], last = rest ? 8.0 + steps * step[(rest + 63) / 64] : 0.0;
+        const double whole = 8.0 + steps * step[height / 32 - 1], last = rest ? 8.0 + steps * step[(rest - 1) / 32] : 0.0;
         us += full * whole + last;
         tiles += full + (rest > 0);
         longest = std::max(longest, full ? whole : last);
     }
     const double each = us / tiles, rounds = tiles / 8 * experts * strips / 256.0;
-    return rounds <= 1 ? longest : rounds * each + 0.7 * longest;
+    // (near one round it may as well be two)
+    return rounds <= 1 ? longest + std::max(0.0, rounds - 0.9) * 3 * each : rounds * each + 0.7 * longest;
 }
 static ExpertsPlan plan_experts(const int4mm_experts_shape& sh) {
     const int64_t pairs = sh.tokens * sh.top_k, K = sh.in_size, F = sh.width;
@@ -579,7 +580,7 @@ static ExpertsPlan plan_experts(const int4mm_experts_shape& sh) {
     if (p.single || !p.tiles) return p;
     auto height = [&](int64_t strips, int64_t steps) {
         int best = 64;
-        for (int h = 128; h <= 256; h += 64)
+        for (int h : {96, 128, 192, 256})
             if (tiles_us(mean, (int)sh.experts, h, strips, steps) < tiles_us(mean, (int)sh.experts, best, strips, steps)) best = h;
         return best;
     };

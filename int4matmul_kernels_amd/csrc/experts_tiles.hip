@@ -46,6 +46,7 @@ __global__ __launch_bounds__(512, 1) void experts_tile_kernel(ExpertsArgs a) {
     h16* const As[A_STAGES] = {A0, A1, A2, A3, A4, A5};
     const int s0 = tile % a.strips * BN;
     if (b.count <= 64) tile_of_height<BITS, SPARSE, 2, GATED>(a, m, b.first, s0, As, Bs, Lut);
+    else if (b.count <= 96) tile_of_height<BITS, SPARSE, 3, GATED>(a, m, b.first, s0, As, Bs, Lut);
     else if (b.count <= 128) tile_of_height<BITS, SPARSE, 4, GATED>(a, m, b.first, s0, As, Bs, Lut);
     else if (b.count <= 192) tile_of_height<BITS, SPARSE, 6, GATED>(a, m, b.first, s0, As, Bs, Lut);
     else tile_of_height<BITS, SPARSE, 8, GATED>(a, m, b.first, s0, As, Bs, Lut);
