@@ -141,13 +141,13 @@ __device__ __forceinline__ h16x8 dequant_chunk(uint32_t bits, const C& c) {
 
 // 16:32 sparse int4.  `v` holds the (up to 8) kept codes of one 8-row chunk as
 // consecutive nibbles, `m8` the chunk's mask bits.  A 256-entry table in LDS
-// (8 words per mask byte: four words of per-half keep masks, two v_perm
-// selectors) spreads the kept codes to their rows: the even / odd nibbles are
+// (per mask byte four words of per-half keep masks and, in a table of their own so that lanes
+// with different bytes meet on fewer banks, two v_perm selectors) spreads the kept codes to their rows: the even / odd nibbles are
 // separated into bytes, v_perm picks for every row the byte of its rank.  Dropped rows
 // are cleared at the end, so they are exactly zero.
-constexpr int SPARSE_LUT_WORDS = 256 * 8;
+constexpr int SPARSE_LUT_WORDS = 256 * 6, SPARSE_LUT_SELECTORS = 256 * 4;
 
-__device__ __forceinline__ void sparse_lut_entry(uint32_t e, uint32_t out[8]) {
+__device__ __forceinline__ void sparse_lut_entry(uint32_t* lut, uint32_t e) {
     uint32_t sel[2] = {0, 0}, hm[4] = {0, 0, 0, 0};
     uint32_t rank = 0;
 #pragma unroll
@@ -157,14 +157,14 @@ __device__ __forceinline__ void sparse_lut_entry(uint32_t e, uint32_t out[8]) {
         sel[i >> 2] |= byte << (8 * (i & 3));
         if (kept) { hm[i >> 1] |= 0xFFFFu << (16 * (i & 1)); ++rank; }
     }
-    out[0] = hm[0]; out[1] = hm[1]; out[2] = hm[2]; out[3] = hm[3];
-    out[4] = sel[0]; out[5] = sel[1]; out[6] = 0; out[7] = 0;
+    *reinterpret_cast<u32x4*>(lut + e * 4) = u32x4{hm[0], hm[1], hm[2], hm[3]};
+    *reinterpret_cast<u32x2*>(lut + SPARSE_LUT_SELECTORS + e * 2) = u32x2{sel[0], sel[1]};
 }
 
 template <class C>
 __device__ __forceinline__ h16x8 dequant_chunk_sparse(uint32_t v, uint32_t m8, const uint32_t* lut, const C& c) {
-    const u32x4 keep = *reinterpret_cast<const u32x4*>(lut + m8 * 8);
-    const u32x2 sel = *reinterpret_cast<const u32x2*>(lut + m8 * 8 + 4);
+    const u32x4 keep = *reinterpret_cast<const u32x4*>(lut + m8 * 4);
+    const u32x2 sel = *reinterpret_cast<const u32x2*>(lut + SPARSE_LUT_SELECTORS + m8 * 2);
     const uint32_t even = v & 0x0F0F0F0Fu, odd = (v >> 4) & 0x0F0F0F0Fu;
     const u32x4 r = bitcast<u32x4>(weights_of_bytes(__builtin_amdgcn_perm(odd, even, sel.x), __builtin_amdgcn_perm(odd, even, sel.y), c));
     return bitcast<h16x8>(r & keep);             // (dropped rows -> +0)

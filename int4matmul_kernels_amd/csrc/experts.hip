@@ -175,12 +175,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, uint3
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);        // raw, 32-bit data format
 }
 __device__ __forceinline__ void fill_lut(uint32_t* lut, int t, int threads) {
-    for (int e = t; e < 256; e += threads) {
-        uint32_t v[8];
-        sparse_lut_entry(e, v);
-        *reinterpret_cast<u32x4*>(lut + e * 8) = u32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<u32x4*>(lut + e * 8 + 4) = u32x4{v[4], v[5], v[6], v[7]};
-    }
+    for (int e = t; e < 256; e += threads) sparse_lut_entry(lut, e);
     __syncthreads();
 }
 

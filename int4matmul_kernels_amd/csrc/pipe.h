@@ -305,12 +305,7 @@ __device__ __forceinline__ void pipe_tile(const MatmulArgs& a, const int m0, con
         int& any_expo = *reinterpret_cast<int*>(Bs);          // borrowed before the pipeline starts
         __syncthreads();
         if constexpr (SPARSE) {
-            if (t < 256) {
-                uint32_t e[8];
-                sparse_lut_entry(t, e);
-                *reinterpret_cast<u32x4*>(lut + t * 8) = u32x4{e[0], e[1], e[2], e[3]};
-                *reinterpret_cast<u32x4*>(lut + t * 8 + 4) = u32x4{e[4], e[5], e[6], e[7]};
-            }
+            if (t < 256) sparse_lut_entry(lut, t);
         }
         if (t == 0) any_expo = 0;
         __syncthreads();
