@@ -18,6 +18,8 @@ struct ExpertsArgs {
     const int* ids;
     const float* weights;
     h16* outs;
+    int* place;                    // [P]: place of each pair, -1 without an expert
+    int few_pairs;                 // rows_kernel, up: the pairs, where it orders them itself, else 0
     int* arrivals;                 // pairs by themselves: [tokens, strips] workgroups that have stored their sums
     int64_t matrix_stride, mask_stride, scale_stride;   // elements from an expert to the next
     int experts, top_k, K, S;      // S: columns of the matrix (up: 2 F)

@@ -3,8 +3,9 @@
 // e = ids[t, j]; a pair whose id is outside 0 ... E - 1 has no expert and adds nothing.  Sums are fp32; h is rounded to fp16 (it is
 // an operand of the matrix instructions), and so is the result.
 //
-//   plan_kernel     pairs in the order of their experts, stable: where each expert's begin, the pairs, each pair's place
-//   rows_kernel     a product of the pairs of one expert, up to 16 MT at a time, with a strip of 64 columns (many pairs an expert:
+//   plan_kernel     pairs in the order of their experts, stable: where each expert's begin, the pairs, each pair's place (up to 256
+//                   pairs: order_few, at the head of the first product)
+//   rows_kernel     a product of the pairs of one expert, up to 32 at a time, with a strip of 64 columns (many pairs an expert:
 //                   experts_tiles.hip)
 //   combine_kernel  the weighted sum of a token's k results, fp32
 //
@@ -182,8 +183,85 @@ __device__ __forceinline__ void fill_lut(uint32_t* lut, int t, int threads) {
 // ---- a product of up to 32 pairs of one expert with 64 columns, 16 MT of them in a tile's rows.  UP: 32 columns of the gate and the same 32 of the other
 // half; the source row of a pair is its token's, the result h.  Else: 64 columns, source and result by place.
 constexpr int ROWS_HEIGHT = 32, ROWS_WAVES = 4;
+// Few pairs: every workgroup of the first product orders them by itself, from LDS, and finds its block's; the first one writes the order
+// down for the kernels behind.  A launch less: us a call, 16 experts of 2048 x 1408, int4, ordered by plan_kernel / so: 32 pairs 27.9 / 25.9, 180 pairs
+// 30.9 / 29.4, 512 pairs 42.7 / 44.8.
+constexpr int FEW_PAIRS = 256, FEW_EXPERTS = 256;
+struct FewPairs { int ids[FEW_PAIRS], count[FEW_EXPERTS], before[FEW_EXPERTS], order[ROWS_HEIGHT]; };
+struct NoPairs { int order[1]; };
+__device__ __forceinline__ bool order_few(const ExpertsArgs& a, int want, FewPairs& f, Block& b) {
+    constexpr int T = 64 * ROWS_WAVES;
+    static_assert(FEW_EXPERTS <= T);
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    if (t < FEW_EXPERTS) f.count[t] = 0;
+    for (int p = t; p < FEW_PAIRS; p += T) {
+        const int v = p < a.few_pairs ? a.ids[p] : -1;
+        f.ids[p] = (uint32_t)v < (uint32_t)a.experts ? v : -1;
+    }
+    __syncthreads();
+    for (int p = t; p < a.few_pairs; p += T)
+        if (f.ids[p] >= 0) atomicAdd(&f.count[f.ids[p]], 1);
+    __syncthreads();
+    // blocks and pairs of the experts up to each, in the halves of a word
+    int blocks = 0, pairs = 0, skip = 0;
+    bool found = false;
+    for (int e0 = 0; e0 < a.experts; e0 += 64) {
+        const int e = e0 + lane, c = e < a.experts ? f.count[e] : 0, own = (c + ROWS_HEIGHT - 1) / ROWS_HEIGHT << 16 | c;
+        int upto = own;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int o = __shfl_up(upto, d);
+            upto += lane >= d ? o : 0;
+        }
+        if (blockIdx.x == 0 && wave == 0 && e < a.experts) {
+            f.before[e] = pairs + ((upto - own) & 0xFFFF);
+            const_cast<int*>(a.offsets)[e] = f.before[e];
+        }
+        const uint64_t beyond = __builtin_amdgcn_ballot_w64(blocks + (upto >> 16) > want);
+        if (!found && beyond) {
+            const int l = __builtin_ctzll(beyond);
+            const int mine = __builtin_amdgcn_readlane(own, l), lower = __builtin_amdgcn_readlane(upto, l) - mine;
+            skip = (want - blocks - (lower >> 16)) * ROWS_HEIGHT;
+            b.expert = e0 + l;
+            b.first = pairs + (lower & 0xFFFF) + skip;
+            b.count = min(ROWS_HEIGHT, (mine & 0xFFFF) - skip);
+            found = true;
+        }
+        const int all = __builtin_amdgcn_readlane(upto, 63);
+        blocks += all >> 16;
+        pairs += all & 0xFFFF;
+    }
+    if (blockIdx.x == 0) {
+        if (t == 0) const_cast<int*>(a.offsets)[a.experts] = pairs;
+        __syncthreads();
+        for (int p = t; p < a.few_pairs; p += T) {
+            const int v = f.ids[p];
+            int where = -1;
+            if (v >= 0) {
+                where = f.before[v];
+                for (int o = 0; o < p; ++o) where += f.ids[o] == v;
+                const_cast<int*>(a.order)[where] = p;
+            }
+            a.place[p] = where;
+        }
+    }
+    if (!found) return false;
+    if (wave == 0) {
+        int seen = 0;
+        for (int i = 0; i < a.few_pairs; i += 64) {
+            const bool mine = f.ids[i + lane] == b.expert;
+            const uint64_t in = __builtin_amdgcn_ballot_w64(mine);
+            const int at = seen + __builtin_popcountll(in & ((1ull << lane) - 1)) - skip;
+            if (mine && at >= 0 && at < ROWS_HEIGHT) f.order[at] = i + lane;
+            seen += __builtin_popcountll(in);
+        }
+    }
+    __syncthreads();
+    return true;
+}
+
 template <int BITS, bool SPARSE, int MT, bool UP>
-__device__ __forceinline__ void rows_tile(const ExpertsArgs& a, const Block& block, char* const (&Xs)[2], uint32_t* lut) {
+__device__ __forceinline__ void rows_tile(const ExpertsArgs& a, const Block& block, char* const (&Xs)[2], uint32_t* lut, const int* few) {
     using F = RowsFmt<BITS, SPARSE>;
     constexpr int HEIGHT = 16 * MT, WAVES = ROWS_WAVES, DEPTH = 2;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -208,7 +286,8 @@ __device__ __forceinline__ void rows_tile(const ExpertsArgs& a, const Block& blo
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
         const int at = min(8 * i + (lane >> 3), count - 1);             // (rows beyond the last repeat it and are not written)
-        x_off[i] = 2u * ((uint32_t)(UP ? a.order[first + at] / a.top_k : at) * a.K + 8 * ((lane & 7) ^ (lane >> 3)));
+        const int row = !UP ? at : (a.few_pairs ? few[at] : a.order[first + at]) / a.top_k;
+        x_off[i] = 2u * ((uint32_t)row * a.K + 8 * ((lane & 7) ^ (lane >> 3)));
     }
     const uint32_t w_off = 4u * col + packed_row<BITS, SPARSE>(q) * row_bytes, w_off2 = 4u * col + packed_row2<BITS, SPARSE>(q) * row_bytes;
 
@@ -367,10 +446,18 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, 2) void rows_kernel(ExpertsArgs a)
     __shared__ __attribute__((aligned(16))) char X0[STAGE], X1[STAGE];
     __shared__ __attribute__((aligned(16))) uint32_t lut[SPARSE ? SPARSE_LUT_WORDS : 4];
     char* const Xs[2] = {X0, X1};
+    __shared__ std::conditional_t<UP, FewPairs, NoPairs> few;
     Block block;
-    if (find_block(a.offsets, a.experts, ROWS_HEIGHT, blockIdx.x / a.strips, threadIdx.x & 63, block) >= 0) return;
-    if (block.count <= 16) rows_tile<BITS, SPARSE, 1, UP>(a, block, Xs, lut);
-    else rows_tile<BITS, SPARSE, 2, UP>(a, block, Xs, lut);
+    bool here = false, ordered = false;
+    if constexpr (UP)
+        if (a.few_pairs) {
+            ordered = true;
+            here = order_few(a, blockIdx.x / a.strips, few, block);
+        }
+    if (!ordered) here = find_block(a.offsets, a.experts, ROWS_HEIGHT, blockIdx.x / a.strips, threadIdx.x & 63, block) < 0;
+    if (!here) return;
+    if (block.count <= 16) rows_tile<BITS, SPARSE, 1, UP>(a, block, Xs, lut, few.order);
+    else rows_tile<BITS, SPARSE, 2, UP>(a, block, Xs, lut, few.order);
 }
 
 // ---- few pairs, hardly two of them of the same expert: no order, a workgroup takes a pair and 64 columns, two launches in all.
@@ -666,7 +753,9 @@ static int experts_share(int bits, bool sparse, h16* outs, const h16* x, const f
     a.weights = weights;
     a.outs = outs;
     const ExpertsPlan plan = plan_experts(*sh);
-    if (!plan.single)
+    a.place = place;
+    a.few_pairs = !plan.single && !plan.tiles && pairs <= FEW_PAIRS && E <= FEW_EXPERTS ? (int)pairs : 0;
+    if (!plan.single && !a.few_pairs)
         hipLaunchKernelGGL(plan_kernel<false>, dim3(E), dim3(1024), 0, st, a.ids, const_cast<int*>(a.offsets), const_cast<int*>(a.order), place, (int)pairs, E);
     if (const int rc = check_launch("experts_forward")) return rc;
     auto rows_of = [&](int64_t k) { return sparse ? k / 16 : k * bits / 32; };

@@ -277,6 +277,17 @@ def test_layer_and_router_together():
     assert thin.sparse and torch.isfinite(thin(x, weights, ids)).all()
 
 
+@pytest.mark.parametrize("T,n,k", [(2, 5, 3), (85, 9, 3), (128, 16, 2), (257, 16, 1), (64, 256, 4), (64, 257, 4), (255, 256, 1), (86, 300, 3)])
+def test_few_pairs_with_and_without_an_expert(ext, T, n, k):
+    """around the sizes where the pairs are ordered in another way; ids that nobody has; all pairs at one expert"""
+    p = problem(T=T, n=n, k=k, K=128, F=64, seed=T)
+    ids = p["ids"].clone()
+    ids[::3, 0] = n
+    ids[1::5] = -1
+    for which in (p["ids"], ids, torch.full_like(ids, n - 1)):
+        close(forward(ext, p, ids=which), plain(dict(p, ids=torch.where(which < n, which, -1))))
+
+
 def test_refusals(ext):
     p = problem(T=4)
     (um, us, uz, _), (dm, ds, dz, _) = p["up"], p["down"]
