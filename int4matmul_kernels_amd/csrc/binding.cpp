@@ -263,9 +263,9 @@ std::tuple<torch::Tensor, torch::Tensor> route_experts(const torch::Tensor& logi
     TORCH_CHECK(logits.scalar_type() == torch::kHalf || logits.scalar_type() == torch::kFloat, "logits must be fp16 or fp32");
     TORCH_CHECK(scoring == "softmax" || scoring == "sigmoid", "scoring must be \"softmax\" or \"sigmoid\"");
     TORCH_CHECK(group_score == "max" || group_score == "top2", "group_score must be \"max\" or \"top2\"");
-    no_gradient({&logits}, "route_experts");
     const int64_t E = logits.size(-1);
     const bool biased = bias.has_value() && bias->defined();
+    no_gradient({&logits, biased ? &*bias : &logits}, "route_experts");
     if (biased) {
         check_tensor(*bias, "bias", torch::kFloat, dev);
         TORCH_CHECK(bias->dim() == 1 && bias->size(0) == E, "bias must be [", E, "]");
@@ -302,7 +302,7 @@ torch::Tensor experts_forward(uint32_t bits, const torch::Tensor& x, const torch
     if (bits != 4 && bits != 3 && bits != 2) throw std::invalid_argument("Unsupported bit width for experts_forward");
     const c10::Device dev = x.device();
     c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
-    no_gradient({&x, &weights}, "experts_forward");
+    no_gradient({&x, &weights, &up_scales, &up_zeros, &down_scales, &down_zeros}, "experts_forward");
     TORCH_CHECK(x.dim() >= 2, "x must be [..., in_size]");
     TORCH_CHECK(weights.defined() && ids.defined() && weights.sizes() == ids.sizes(), "weights and ids must have the same shape");
     TORCH_CHECK(ids.dim() == x.dim() && ids.sizes().slice(0, ids.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
@@ -370,7 +370,7 @@ torch::Tensor low_rank_add(const torch::Tensor& base, const torch::Tensor& x, co
         check_tensor(*outs, "outs", torch::kHalf, dev);
         TORCH_CHECK(outs->sizes() == base.sizes(), "outs must be ", base.sizes());
         at::assert_no_partial_overlap(*outs, from);
-        for (const auto* t : {&states, &down, &up}) at::assert_no_overlap(*outs, *t);
+        for (const auto* t : {&states, &down, &up, &scales, &ids}) at::assert_no_overlap(*outs, *t);
         to = *outs;
     } else {
         to = at::empty(base.sizes(), torch::TensorOptions().dtype(torch::kHalf).device(dev));

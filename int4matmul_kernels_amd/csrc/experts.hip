@@ -725,8 +725,8 @@ static ExpertsParts experts_parts(const int4mm_experts_shape& sh) {
     p.offsets = 0;
     p.order = p.offsets + round(4 * (size_t)(sh.experts + 1));
     p.place = p.order + round(4 * pairs);
-    p.arrivals = p.place + round(4 * pairs);              // (pairs by themselves: up to 64 tokens)
-    p.h = p.arrivals + (pairs <= 64 ? round(4 * (size_t)(tokens * (sh.in_size / 64))) : 0);
+    p.arrivals = p.place + round(4 * pairs);              // (pairs by themselves: up to 64 tokens, also as the last share of many)
+    p.h = p.arrivals + round(4 * (size_t)(std::min<int64_t>(tokens, 64) * (sh.in_size / 64)));
     p.part = p.h + round(2 * pairs * (size_t)sh.width);
     p.total = p.part + round(4 * pairs * (size_t)sh.in_size);
     return p;

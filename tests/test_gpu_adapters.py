@@ -306,3 +306,15 @@ def test_rows_in_order_leave_what_lies_behind(ext):
     with pytest.raises(capi.Int4mmError) as e:
         capi.low_rank_add(outs[:500], p["base"][:, 0], p["x"][:, 0], p["down"], p["up"], p["scales"], p["ids"], 1, ws[:-16])
     assert e.value.code == 6
+
+
+def test_outs_over_scales_or_ids_is_refused(ext):
+    p = problem((4, 2), 1024, 1, 64, 64)
+    raw = torch.zeros(4096, dtype=torch.uint8, device="cuda")
+    outs = raw[:1024].view(torch.float16).reshape(4, 2, 64)
+    scales = raw.view(torch.float32)[:1024]
+    with pytest.raises(RuntimeError):
+        ext.low_rank_add(p["base"], p["x"], p["down"], p["up"], scales, p["ids"], outs=outs)
+    ids = raw.view(torch.int32)[:4]
+    with pytest.raises(RuntimeError):
+        ext.low_rank_add(p["base"], p["x"], p["down"], p["up"], p["scales"], ids, outs=outs)

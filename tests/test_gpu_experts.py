@@ -240,6 +240,19 @@ def test_offsets_beyond_32_bits(ext):
         close(got[rows], plain(dict(p, x=x[rows], ids=ids[rows], weights=weights[rows])))
 
 
+def test_a_last_share_of_one_token(ext):
+    """so many pairs that they go through the workspace in shares, the last one with a token alone"""
+    T, k = 4096 * 4095 + 1, 64
+    p = problem(T=1, n=70, k=64, K=64, F=64, seed=6)
+    x = torch.zeros((T, 64), dtype=torch.float16, device="cuda")
+    ids = torch.full((T, k), -1, dtype=torch.int32, device="cuda")
+    weights = torch.zeros((T, k), device="cuda")
+    x[-1:], ids[-1:], weights[-1:] = p["x"], p["ids"], p["weights"]
+    got = forward(ext, p, x=x, ids=ids, weights=weights)
+    assert torch.equal(got[-1:], forward(ext, p)) and not got[:-1].any()
+    close(got[-1:], plain(p))
+
+
 def test_layer_and_router_together():
     """router, experts and the modules that hold them, as a block of a model uses them"""
     from int4matmul_kernels_amd.quant_experts import ExpertRouter, QuantExperts

@@ -198,3 +198,8 @@ def test_refusals(ext):
         ext.route_experts(asks, 2)
     with torch.no_grad():
         ext.route_experts(asks, 2)
+
+
+def test_a_bias_that_asks_for_a_gradient_is_refused(ext):
+    with pytest.raises(RuntimeError, match="no backward"):
+        ext.route_experts(logits_of(4, 32, torch.float16, 5), 2, bias=torch.zeros(32, device="cuda", requires_grad=True))
