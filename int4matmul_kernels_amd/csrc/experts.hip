@@ -161,15 +161,16 @@ __device__ __forceinline__ uint32_t packed_row(int q) { return BITS == 4 && !SPA
 template <int BITS, bool SPARSE>
 __device__ __forceinline__ uint32_t packed_row2(int q) { return SPARSE ? 1u : min(packed_row<BITS, SPARSE>(q) + 1u, 2u); }
 
-// (A, B) of sum x w = A sum x value + B sum x
+// (A, B) of sum x w = A sum x value + B sum x.  (16:32 and a NaN scale: A is that NaN, since `value` may come from the linear decode, which
+// has not met the scale; see any_negative)
 template <bool SPARSE>
 __device__ __forceinline__ void fold_factors(uint32_t s2, uint32_t z2, int odd, float& A, float& B) {
     const float s = (float)as_h2(s2)[odd], z = (float)as_h2(z2)[odd];
     const bool linear = s >= 0.f;
-    A = linear ? s : SPARSE ? 1.f : -s;
+    A = linear ? s : SPARSE ? (s < 0.f ? 1.f : s) : -s;
     B = linear ? -s * z : z;
 }
-// a negative or NaN scale anywhere in the wave: the decode that serves either mode
+// a scale with its sign set anywhere in the wave: the decode that serves either mode
 __device__ __forceinline__ bool any_negative(uint32_t a, uint32_t b) { return __builtin_amdgcn_ballot_w64(((a | b) & 0x80008000u) != 0) != 0; }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, uint32_t bytes) {

@@ -316,3 +316,28 @@ def test_refusals(ext):
         forward(ext, p, bits=5)
     with pytest.raises(RuntimeError, match="no backward"):
         forward(ext, p, x=p["x"].clone().requires_grad_())
+
+
+@pytest.mark.parametrize("bits,sparse", FORMATS)
+@pytest.mark.parametrize("T,n", [(1, 4), (9, 4), (300, 16), (300, 4)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_a_single_nan_scale(ext, bits, sparse, T, n, sign):
+    """one group of one column of one expert has a NaN scale, of either sign: NaN where the definition has it, all else as without"""
+    p = problem(bits, sparse, n, 1, T, seed=T + bits)
+    ids = p["ids"].clone()
+    ids[0] = 2
+    nan = torch.tensor([0x7E00 if sign > 0 else -0x200], dtype=torch.int16, device="cuda").view(torch.float16)
+    F = p["wd"].shape[1]
+    for which, column, rows in (("up", 5, slice(64, 128)), ("up", F + 70, slice(64, 128)), ("down", 133, slice(64, 128))):
+        m, s, z, k = p[which]
+        s = s.clone()
+        s[2, 1, column] = nan[0]
+        assert s.view(torch.int16)[2, 1, column] == nan.view(torch.int16)[0]
+        exact = p["w" + which[0]].clone()
+        exact[2, rows, column] = math.nan
+        got = forward(ext, p, ids=ids, **{which: (m, s, z, k)})
+        want = plain(dict(p, ids=ids, **{"w" + which[0]: exact}))
+        assert want[0].isnan().any() and torch.equal(got.isnan(), want.isnan())
+        there = ~want.isnan()
+        if there.any():
+            close(got[there], want[there])
