@@ -13,7 +13,7 @@ struct ExpertsArgs {
     const h16* zeros;
     const int* offsets;            // [E + 1]: an expert's pairs among the ordered ones
     const int* order;              // [P]: pair of each place
-    h16* h;                        // up: [P, F] by place; tiles of the second product: [P, S]
+    h16* h;                        // up: [P, F] by place
     float* part;                   // down: [P, S] by place
     const int* ids;
     const float* weights;

@@ -604,29 +604,26 @@ __global__ __launch_bounds__(512) void token_kernel(ExpertsArgs a) {
     }
 }
 
-// outs[t, :] = sum over j of weights[t, j] part[place[t, j], :]; a thread takes four columns (fp32) or eight (fp16)
-template <typename T>
-__global__ __launch_bounds__(256) void combine_kernel(h16* outs, const T* part, const float* weights, const int* place, int top_k, int S, int parts) {
-    constexpr int N = 16 / sizeof(T);
-    typedef T Vec __attribute__((ext_vector_type(N)));
-    typedef h16 Out __attribute__((ext_vector_type(N)));
+// outs[t, :] = sum over j of weights[t, j] part[place[t, j], :]; a thread takes four columns
+__global__ __launch_bounds__(256) void combine_kernel(h16* outs, const float* part, const float* weights, const int* place, int top_k, int S, int parts) {
+    constexpr int N = 4;
     const int64_t t = blockIdx.x / parts;
     const int c = ((int)(blockIdx.x % parts) * 256 + threadIdx.x) * N;
     if (c >= S) return;
-    float sum[N] = {};
+    f32x4 sum = {};
 #pragma unroll 4
     for (int j = 0; j < top_k; ++j) {
         const int p = place[t * top_k + j];
         if (p < 0) continue;
         const float w = weights[t * top_k + j];
-        const Vec v = *reinterpret_cast<const Vec*>(part + (int64_t)p * S + c);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(part + (int64_t)p * S + c);
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] += w * (float)v[i];
+        for (int i = 0; i < N; ++i) sum[i] += w * v[i];
     }
-    Out o;
+    h16x4 o;
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = (h16)sum[i];
-    *reinterpret_cast<Out*>(outs + t * S + c) = o;
+    *reinterpret_cast<h16x4*>(outs + t * S + c) = o;
 }
 
 // ---- which kernels, by the pairs of an expert if all are asked alike (the host does not know how they are shared out).
@@ -789,20 +786,11 @@ static int experts_share(int bits, bool sparse, h16* outs, const h16* x, const f
         token_product<false>(bits, a, pairs, st);
         return check_launch("experts_forward");
     }
-    if (plan.tiles) {
-        a.h = reinterpret_cast<h16*>(ws + parts.part);
-        launch_experts_tiles(bits, a, plan.down, pairs, false, st);
-    } else {
-        rows_product<false>(bits, a, pairs, st);
-    }
+    if (plan.tiles) launch_experts_tiles(bits, a, plan.down, pairs, false, st);
+    else rows_product<false>(bits, a, pairs, st);
     if (const int rc = check_launch("experts_forward")) return rc;
-    const int columns = (int)((K + (plan.tiles ? 2047 : 1023)) / (plan.tiles ? 2048 : 1024));
-    const dim3 grid((unsigned)(sh->tokens * columns));
-    if (plan.tiles)
-        hipLaunchKernelGGL(combine_kernel<h16>, grid, dim3(256), 0, st, a.outs, a.h, a.weights, place,
-                           a.top_k, (int)K, columns);
-    else
-        hipLaunchKernelGGL(combine_kernel<float>, grid, dim3(256), 0, st, a.outs, a.part, a.weights, place, a.top_k, (int)K, columns);
+    const int columns = (int)((K + 1023) / 1024);
+    hipLaunchKernelGGL(combine_kernel, dim3((unsigned)(sh->tokens * columns)), dim3(256), 0, st, a.outs, a.part, a.weights, place, a.top_k, (int)K, columns);
     return check_launch("experts_forward");
 }
 

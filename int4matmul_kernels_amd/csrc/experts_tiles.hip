@@ -3,8 +3,9 @@
 // activation, so that neither a gathered copy of x nor the gate's and the other half's results pass through memory; the second one
 // takes the pairs as they lie.
 //
-// Weights are rounded to fp16 as int4mm_dequantize's are, and a pair's result once more: sums of exact codes would need a group's sums beside the
-// running ones, twice 128 of the 256 registers that a lane has.
+// Weights are rounded to fp16 as int4mm_dequantize's are: sums of exact codes would need a group's sums beside the running ones, twice 128 of
+// the 256 registers that a lane has.  A pair's result is stored in fp32, as those of rows_kernel are: its weight, which may be what brings it into
+// fp16's range, comes after it.  (In fp16 calls took 2 - 12 % less, 16:32 experts gaining most, and a result beyond 65504 was lost.)
 //
 // What bounds it: large batches the power limit (4096 tokens, eight of 64 experts of 2048 x 1024, int4: 282 and 164 us for 275 and 137 GFLOP, tiles' rows beyond
 // an expert's last one included 1.1 PFLOP/s); few rows the chain of a step, 0.44 us whatever the height.  One height for all of a launch's blocks instead: 510 us a
@@ -21,7 +22,7 @@ __device__ __forceinline__ void tile_of_height(const ExpertsArgs& a, const Matmu
         pipe_tile<BITS, SPARSE, TM, 4, true, false, true>(m, 0, s0, a.x, a.h + (int64_t)first * (a.S / 2), As, Bs, lut, 0, 0, 1,
                                                           GatedRows{a.order + first, a.top_k, a.S / 2, a.x_bytes});
     else
-        pipe_tile<BITS, SPARSE, TM, 4, true, false>(m, 0, s0, a.x + (int64_t)first * a.K, a.h + (int64_t)first * a.S, As, Bs, lut, 0, 0, 1);
+        pipe_tile<BITS, SPARSE, TM, 4, true, false, false, float>(m, 0, s0, a.x + (int64_t)first * a.K, a.part + (int64_t)first * a.S, As, Bs, lut, 0, 0, 1);
 }
 
 // A block of fewer rows than the launch's height takes the lowest tile that holds it, so that what is computed beyond an expert's last

@@ -83,9 +83,10 @@ __device__ __forceinline__ float silu_times(float gate, float up) { return gate 
 
 // PING: the waves of the first half run phase 0, MFMAs first and then everything else; those of the second half phase 1,
 // everything else first and the MFMAs last.  Without it all waves run phase 1.
-template <int BITS, bool SPARSE, int TM, int NW, bool PING, bool SPLIT, bool GATED = false>
+// Out: what the results are stored as, h16 or float.
+template <int BITS, bool SPARSE, int TM, int NW, bool PING, bool SPLIT, bool GATED = false, class Out = h16>
 __device__ __forceinline__ void pipe_tile(const MatmulArgs& a, const int m0, const int s0, const h16* x,
-                                          h16* outs, h16* const (&As)[A_STAGES], h16* Bs, uint32_t* lut, const int tile, const int split,
+                                          Out* outs, h16* const (&As)[A_STAGES], h16* Bs, uint32_t* lut, const int tile, const int split,
                                           const int nsplit, const GatedRows gated = {}) {
     constexpr int BM = TM * 32, BN = NW * 64, WM = TM * 16, WN = 64, TN = 4, T = 2 * NW * 64;
     constexpr int A_ROWS = T / 4;                                  // rows covered by one 16-byte load per thread
@@ -486,15 +487,16 @@ __device__ __forceinline__ void pipe_tile(const MatmulArgs& a, const int m0, con
     }
     if (s0 + wn0 >= a.S) return;                       // (a wave's 64 columns are inside or outside as one)
     // register r of tile (i, j) is row 16 i + 4 (lane / 16) + r, column 4 (lane % 16) + j of the wave's
-    h16* const out = outs + (int64_t)(m0 + wm0 + 4 * (lane >> 4)) * a.S + s0 + wn0 + 4 * (lane & 15);
+    typedef Out Out4 __attribute__((ext_vector_type(4)));
+    Out* const out = outs + (int64_t)(m0 + wm0 + 4 * (lane >> 4)) * a.S + s0 + wn0 + 4 * (lane & 15);
     const int rows = a.M - (m0 + wm0 + 4 * (lane >> 4));
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (16 * i + r < rows)
-                *reinterpret_cast<h16x4*>(out + (int64_t)(16 * i + r) * a.S) =
-                    h16x4{(h16)acc[i][0][r], (h16)acc[i][1][r], (h16)acc[i][2][r], (h16)acc[i][3][r]};
+                *reinterpret_cast<Out4*>(out + (int64_t)(16 * i + r) * a.S) =
+                    Out4{(Out)acc[i][0][r], (Out)acc[i][1][r], (Out)acc[i][2][r], (Out)acc[i][3][r]};
 }
 
 }  // namespace i4

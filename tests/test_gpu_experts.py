@@ -341,3 +341,19 @@ def test_a_single_nan_scale(ext, bits, sparse, T, n, sign):
         there = ~want.isnan()
         if there.any():
             close(got[there], want[there])
+
+
+@pytest.mark.parametrize("bits,sparse", FORMATS)
+@pytest.mark.parametrize("T", [20, 300, 900])
+def test_pairs_beyond_the_range_of_fp16(ext, bits, sparse, T):
+    """h @ DOWN far above 65504, weights that bring a token's sum back: the same in a small batch and in a large one"""
+    p = problem(bits, sparse, 3, 2, T, seed=T)
+    (m, s, z, k), by = p["down"], 2.0 ** 18 if bits == 4 else 2.0 ** 17
+    p["down"], p["wd"] = (m, (s.float() * by).half(), z, k), p["wd"] * by
+    p["weights"] = p["weights"] * 2.0 ** -16 * torch.tensor([1.0, -1.0], device="cuda")
+    h = dict(p, weights=torch.tensor([1.0, 0.0], device="cuda").expand(T, 2))
+    assert plain(h).abs().max() > 65504
+    got = forward(ext, p)
+    close(got, plain(p))
+    if T > 20:
+        assert (got[:3].double() - forward(ext, p, x=p["x"][:3], ids=p["ids"][:3], weights=p["weights"][:3]).double()).norm() <= 2 * REL * got[:3].double().norm()
