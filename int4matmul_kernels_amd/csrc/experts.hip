@@ -658,14 +658,15 @@ static ExpertsPlan plan_experts(const int4mm_experts_shape& sh) {
     const double mean = (double)pairs / sh.experts;
     ExpertsPlan p{pairs <= 64 && (sh.tokens == 1 || 2 * pairs <= sh.experts), mean > 40, 128, 128};
     if (p.single || !p.tiles) return p;
-    auto height = [&](int64_t strips, int64_t steps) {
+    // (`row`: of the second product, whose tiles address their rows with 31 bits; 64 rows of any width that check_experts admits)
+    auto height = [&](int64_t strips, int64_t steps, int64_t row) {
         int best = 64;
         for (int h : {96, 128, 192, 256})
-            if (tiles_us(mean, (int)sh.experts, h, strips, steps) < tiles_us(mean, (int)sh.experts, best, strips, steps)) best = h;
+            if (2 * h * row < (int64_t)1 << 31 && tiles_us(mean, (int)sh.experts, h, strips, steps) < tiles_us(mean, (int)sh.experts, best, strips, steps)) best = h;
         return best;
     };
-    p.up = height((F + 127) / 128, K / 32);
-    p.down = height((K + 255) / 256, F / 32);
+    p.up = height((F + 127) / 128, K / 32, 0);
+    p.down = height((K + 255) / 256, F / 32, F);
     return p;
 }
 
@@ -706,7 +707,7 @@ static int check_experts(int bits, const int4mm_experts_shape* sh, bool sparse) 
     if (g == 0 || (g > 0 && g % 64 != 0)) return INT4MM_ERR_GROUP;
     const int64_t up_groups = g < 0 ? 1 : (K + g - 1) / g, down_groups = g < 0 ? 1 : (F + g - 1) / g;
     if (sh->up_groups != up_groups || sh->down_groups != down_groups) return INT4MM_ERR_SHAPE;
-    // (a matrix, and the rows of a block, are addressed with 31 bits)
+    // (a matrix, and 64 rows, are addressed with 31 bits)
     if (K >= limit / 128 || F >= limit / 128 || K * F >= limit) return INT4MM_ERR_SHAPE;
     if (sh->top_k > 1024 || sh->tokens >= limit) return INT4MM_ERR_SHAPE;
     // (a grid of one dimension has a workgroup for every 32 pairs, or expert, and 64 columns)

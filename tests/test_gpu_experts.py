@@ -357,3 +357,19 @@ def test_pairs_beyond_the_range_of_fp16(ext, bits, sparse, T):
     close(got, plain(p))
     if T > 20:
         assert (got[:3].double() - forward(ext, p, x=p["x"][:3], ids=p["ids"][:3], weights=p["weights"][:3]).double()).norm() <= 2 * REL * got[:3].double().norm()
+
+
+def test_the_widest_rows(ext):
+    """a width where a tile of 256 rows would be 2^32 bytes of hidden states"""
+    T, F, part = 300, 2 ** 23, 2 ** 17
+    p, gen = problem(2, False, 1, 1, T, 64, 64, -1, seed=8), torch.Generator(device="cuda").manual_seed(8)
+    p["up"], p["wu"] = packed(2, False, 1, 64, 2 * F, -1, gen)
+    parts = [packed(2, False, 1, part, 64, -1, gen) for _ in range(F // part)]         # (a matrix is packed in parts of its rows)
+    first = parts[0][0]
+    p["down"] = (torch.cat([m for (m, _, _, _), _ in parts], dim=1), first[1], first[2], None)
+    p["wd"] = torch.cat([w / s.double() * first[1].double() for (_, s, _, _), w in parts], dim=1)
+    got = forward(ext, p)
+    for rows in (slice(0, 3), slice(255, 258), slice(T - 3, T)):
+        close(got[rows], plain(dict(p, x=p["x"][rows], ids=p["ids"][rows], weights=p["weights"][rows])))
+    few = forward(ext, p, x=p["x"][:20], ids=p["ids"][:20], weights=p["weights"][:20])
+    close(few[:3], plain(dict(p, x=p["x"][:3], ids=p["ids"][:3], weights=p["weights"][:3])))
