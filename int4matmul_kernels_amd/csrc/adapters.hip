@@ -510,10 +510,15 @@ int int4mm_low_rank_add(void* outs, const void* base, const void* x, const void*
     const int height = 16 * p.mt;
     const dim3 grid((unsigned)((sh->out_size + 256 * p.strips - 1) / (256 * p.strips)), (unsigned)p.tiles, (unsigned)p.deal_expand);
     const size_t lds = (size_t)height * (((sh->rank + 31) / 32 * 32 + 8) * 4 + 4);
-#define EXPAND_AS(MT, SORTED)                                                                                        \
-    if (sh->rank <= 32) hipLaunchKernelGGL((expand_kernel<MT, false, 1, SORTED>), grid, dim3(256), lds, st, a);      \
-    else if (sh->rank <= 64) hipLaunchKernelGGL((expand_kernel<MT, false, 2, SORTED>), grid, dim3(256), lds, st, a); \
-    else hipLaunchKernelGGL((expand_kernel<MT, true, 2, SORTED>), grid, dim3(256), lds, st, a)
+    auto expand = [&](void (*kernel)(AdapterArgs)) {
+        // more than 64 KB of dynamic LDS (32 rows of more than 480 ranks) has to be requested
+        if (lds > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a);
+    };
+#define EXPAND_AS(MT, SORTED)                                               \
+    if (sh->rank <= 32) expand(expand_kernel<MT, false, 1, SORTED>);        \
+    else if (sh->rank <= 64) expand(expand_kernel<MT, false, 2, SORTED>);   \
+    else expand(expand_kernel<MT, true, 2, SORTED>)
 #define EXPAND(MT) if (p.sorted) { EXPAND_AS(MT, true); } else { EXPAND_AS(MT, false); }
     if (p.mt == 1) { EXPAND(1) }
     else { EXPAND(2) }

@@ -318,3 +318,19 @@ def test_outs_over_scales_or_ids_is_refused(ext):
     ids = raw.view(torch.int32)[:4]
     with pytest.raises(RuntimeError):
         ext.low_rank_add(p["base"], p["x"], p["down"], p["up"], p["scales"], ids, outs=outs)
+
+
+@pytest.mark.parametrize("rank", [480, 481, 512])
+@pytest.mark.parametrize("shape,per_row,n", [((3, 401), False, 3), ((1, 1203), True, 9), ((1, 1025), True, 1)])
+def test_highest_ranks_with_many_rows(ext, rank, shape, per_row, n):
+    """tiles of 32 rows whose x down^T takes more than 64 KB of LDS"""
+    p = problem(shape, n, rank, 128, 320, per_row=per_row, seed=rank)
+    close(add(ext, p), p)
+    if rank == 512:
+        held, graph = {k: v.clone() for k, v in p.items()}, torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = add(ext, held)
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, add(ext, p))
