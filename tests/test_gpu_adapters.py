@@ -334,3 +334,19 @@ def test_highest_ranks_with_many_rows(ext, rank, shape, per_row, n):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, add(ext, p))
+
+
+@pytest.mark.parametrize("rank", [16, 20, 33, 64, 100, 200, 512])
+@pytest.mark.parametrize("shape,n", [((3, 401), 4), ((5, 333), 2), ((70, 17), 9), ((2, 1024), 3)])
+def test_prompts_of_many_rows(ext, rank, shape, n):
+    """an id per request and more than 1024 rows: tiles of 32 rows that several requests share, idle ones among them, a last tile that is
+    not full; in place too"""
+    p = problem(shape, n, rank, 192, 320, seed=rank)
+    p["ids"][-1] = n - 1
+    p["ids"][1] = -1
+    got = add(ext, p)
+    close(got, p)
+    assert torch.equal(got[1], p["base"][1])
+    base = p["base"].clone()
+    ext.low_rank_add(base, p["x"], p["down"], p["up"], p["scales"], p["ids"], base)
+    assert torch.equal(base, got)
