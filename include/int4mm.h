@@ -289,8 +289,9 @@ INT4MM_API int int4mm_route_experts(void* weights, void* ids, const void* logits
  * adds nothing (its weight is not looked at); a token without a pair gets 0.  The same expert may be named twice.  Sums are fp32;
  * up to 40 pairs an expert, if all are asked alike, exact codes are multiplied (16:32: codes less their zero, rounded once) and
  * scale and zero applied to the sums, beyond that int4mm_dequantize's weights.  Results are a deterministic function of the arguments.
- * K and F multiples of 64, K F < 2^31, at most 4096 experts and 1024 slots a token.  The workspace holds what up to 2^18 pairs at a
- * time need; more go through it in shares. */
+ * K and F multiples of 64 below 2^24, K F < 2^31, at most 4096 experts and 1024 slots a token (fewer where K or F is beyond a million: a grid
+ * has fewer than 2^32 work-items, 512 for a pair and 64 columns).  The workspace holds what up to 2^18 pairs at a time need; more go
+ * through it in shares. */
 typedef struct int4mm_experts_shape {
     int64_t tokens, top_k, experts;
     int64_t in_size;       /* K */

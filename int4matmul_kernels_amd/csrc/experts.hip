@@ -690,10 +690,27 @@ static void token_product(int bits, ExpertsArgs a, int64_t pairs, hipStream_t st
     else hipLaunchKernelGGL((token_kernel<2, false, UP>), grid, block, 0, st, a);
 }
 
-// Tokens that go through the launches at once, in even shares: their states are addressed with 31 bits, and of many pairs (a quarter
-// of a million fill the GPU many times over) not all need a workspace at the same time.
+// work-items of the largest grid that a call of so few tokens launches
+static int64_t work_items(const int4mm_experts_shape& sh) {
+    const ExpertsPlan plan = plan_experts(sh);
+    const int64_t pairs = sh.tokens * sh.top_k, E = sh.experts, K = sh.in_size, F = sh.width;
+    if (plan.single) return pairs * (std::max(K, 2 * F) / 64) * 512;
+    if (!plan.tiles) return std::min(pairs, E + pairs / ROWS_HEIGHT) * (std::max(K, 2 * F) / 64) * (64 * ROWS_WAVES);
+    auto tiles = [&](int height, int64_t S) { return (std::min(pairs, E + pairs / height) * ((S + 255) / 256) + 7) * 512; };
+    return std::max(tiles(plan.up, 2 * F), tiles(plan.down, K));
+}
+
+// Tokens that go through the launches at once, in even shares: their states are addressed with 31 bits, of many pairs (a quarter
+// of a million fill the GPU many times over) not all need a workspace at the same time, and a grid has fewer than 2^32 work-items.
+constexpr int64_t PAIRS_AT_ONCE = (int64_t)1 << 18, GRID_ITEMS = ((int64_t)1 << 32) - 4096;
 static int64_t tokens_at_once(const int4mm_experts_shape& sh) {
-    const int64_t most = std::max<int64_t>(1, std::min((((int64_t)1 << 31) - 1) / (2 * sh.in_size), ((int64_t)1 << 18) / sh.top_k));
+    int64_t most = std::max<int64_t>(1, std::min((((int64_t)1 << 31) - 1) / (2 * sh.in_size), PAIRS_AT_ONCE / sh.top_k));
+    // (the most that any number of pairs takes: blocks up to a mean of 40, the lowest tiles, 64 pairs by themselves; a pair never takes
+    // more than 512 work-items a strip)
+    const int64_t E = sh.experts, strips = std::max(sh.in_size, 2 * sh.width) / 64;
+    if ((E + std::min(PAIRS_AT_ONCE, 40 * E) / ROWS_HEIGHT) * strips * (64 * ROWS_WAVES) > GRID_ITEMS ||
+        (E + PAIRS_AT_ONCE / 64) * ((strips + 3) / 4) * 512 > GRID_ITEMS || 64 * strips * 512 > GRID_ITEMS)
+        most = std::min(most, std::max<int64_t>(1, GRID_ITEMS / (strips * 512) / sh.top_k));
     const int64_t shares = (sh.tokens + most - 1) / most;
     return shares <= 1 ? sh.tokens : (sh.tokens + shares - 1) / shares;
 }
@@ -710,8 +727,12 @@ static int check_experts(int bits, const int4mm_experts_shape* sh, bool sparse) 
     // (a matrix, and 64 rows, are addressed with 31 bits)
     if (K >= limit / 128 || F >= limit / 128 || K * F >= limit) return INT4MM_ERR_SHAPE;
     if (sh->top_k > 1024 || sh->tokens >= limit) return INT4MM_ERR_SHAPE;
-    // (a grid of one dimension has a workgroup for every 32 pairs, or expert, and 64 columns)
-    if ((tokens_at_once(*sh) * sh->top_k / 16 + sh->experts) * (std::max(K, 2 * F) / 64) >= limit) return INT4MM_ERR_SHAPE;
+    // (where even a token's grid is too large)
+    if (tokens_at_once(*sh) == 1) {
+        int4mm_experts_shape one = *sh;
+        one.tokens = 1;
+        if (work_items(one) > GRID_ITEMS) return INT4MM_ERR_SHAPE;
+    }
     return INT4MM_OK;
 }
 

@@ -116,3 +116,26 @@ def test_modules_refuse():
     for how in ((0, 4, 64, 64), (2, 0, 64, 64), (2, 513, 64, 64), (2, 4, 65, 64)):
         with pytest.raises(ValueError):
             LowRankAdapters(*how, device="cpu")
+
+
+def test_experts_grids():
+    """a grid has fewer than 2^32 work-items: so many pairs go through in shares, and a token that is too much by itself is refused"""
+    lib = capi.lib()
+
+    def call(*shape):
+        ptrs = [OK] * 12
+        ptrs[7] = ptrs[11] = None
+        sh = capi.experts_shape(*shape)
+        return lib.int4mm_experts_forward(4, *map(VP, ptrs), C.byref(sh), VP(OK), 0, None), lib.int4mm_experts_workspace_bytes(C.byref(sh))
+
+    # (no workspace is given: 6 is an accepted shape)
+    widest = (1 << 24) - 64
+    assert call(1, 64, 128, 64, widest, -1) == (3, 0) and call(7, 17, 128, 64, widest, -1) == (3, 0)
+    assert call(1, 16, 128, 64, widest, -1)[0] == 6 and call(7, 16, 128, 64, widest, -1)[0] == 6
+    # 1000 tokens, one of 4096 experts each, 32768 strips of columns: 256 work-items for each, 8.6e9 in one grid
+    code, size = call(1000, 1, 4096, 64, 1 << 20, -1)
+    assert code == 6 and size < 256 * 2 ** 21 * 1.01
+    # ordinary ones are not cut: the hidden states of all pairs, their sums, and a little
+    for T, k, E, K, F in ((4096, 8, 64, 2048, 1024), (8192, 2, 8, 4096, 14336), (32768, 8, 256, 7168, 2048), (2048, 4, 16, 4096, 32768)):
+        code, size = call(T, k, E, K, F, 128)
+        assert code == 6 and T * k * (2 * F + 4 * K) < size < 1.02 * T * k * (2 * F + 4 * K + 8) + 2 ** 20

@@ -373,3 +373,25 @@ def test_the_widest_rows(ext):
         close(got[rows], plain(dict(p, x=p["x"][rows], ids=p["ids"][rows], weights=p["weights"][rows])))
     few = forward(ext, p, x=p["x"][:20], ids=p["ids"][:20], weights=p["weights"][:20])
     close(few[:3], plain(dict(p, x=p["x"][:3], ids=p["ids"][:3], weights=p["weights"][:3])))
+
+
+def test_more_work_items_than_a_grid_has(ext):
+    """1000 pairs, one of 4096 experts each, of 2^21 columns: 8.6e9 work-items if they were one launch.  (The first eight experts are asked,
+    and only they are in memory.)"""
+    import ctypes as C
+    from int4matmul_kernels_amd import capi
+    T, K, F, part = 1000, 64, 2 ** 20, 2 ** 17
+    p, gen = problem(2, False, 8, 1, T, 64, 64, -1, seed=9), torch.Generator(device="cuda").manual_seed(9)
+    p["up"], p["wu"] = packed(2, False, 8, 64, 2 * F, -1, gen)
+    parts = [packed(2, False, 8, part, 64, -1, gen) for _ in range(F // part)]
+    first = parts[0][0]
+    p["down"] = (torch.cat([m for (m, _, _, _), _ in parts], dim=1), first[1], first[2], None)
+    p["wd"] = torch.cat([w / s.double() * first[1].double() for (_, s, _, _), w in parts], dim=1)
+    sh = capi.experts_shape(T, 1, 4096, K, F, -1)
+    ws = torch.empty(capi.lib().int4mm_experts_workspace_bytes(C.byref(sh)), dtype=torch.uint8, device="cuda")
+    outs = torch.empty((T, K), dtype=torch.float16, device="cuda")
+    ptr = lambda t: C.c_void_p(None if t is None else t.data_ptr())
+    assert capi.lib().int4mm_experts_forward(2, *map(ptr, (outs, p["x"], p["weights"], p["ids"], *p["up"], *p["down"])), C.byref(sh), ptr(ws), ws.numel(),
+                                             C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    for rows in (slice(0, 4), slice(254, 258), slice(T // 2, T // 2 + 4), slice(T - 4, T)):
+        close(outs[rows], plain(dict(p, x=p["x"][rows], ids=p["ids"][rows], weights=p["weights"][rows])))
