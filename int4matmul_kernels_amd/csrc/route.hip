@@ -193,18 +193,28 @@ __global__ __launch_bounds__(256) void route_kernel(const L* logits, RouteArgs a
     }
 }
 
+constexpr int64_t ROUTE_AT_ONCE = (int64_t)1 << 25;      // tokens of a launch: a grid has fewer than 2^32 work-items, 64 for a token
+
 template <bool BIAS, typename L>
-static void launch_route(const L* logits, const RouteArgs& a, hipStream_t st) {
-    // one wave a workgroup where that still leaves CUs without one, else four
-    const int waves = a.tokens <= 512 ? 1 : 4;
-    const dim3 grid((unsigned)((a.tokens + waves - 1) / waves)), block(64 * waves);
-    const size_t lds = a.groups > 1 ? (size_t)waves * a.experts * sizeof(double) : 0;
-    const int epl = (a.experts + 63) / 64;
-    if (epl <= 1) hipLaunchKernelGGL((route_kernel<1, BIAS, L>), grid, block, lds, st, logits, a);
-    else if (epl <= 2) hipLaunchKernelGGL((route_kernel<2, BIAS, L>), grid, block, lds, st, logits, a);
-    else if (epl <= 4) hipLaunchKernelGGL((route_kernel<4, BIAS, L>), grid, block, lds, st, logits, a);
-    else if (epl <= 8) hipLaunchKernelGGL((route_kernel<8, BIAS, L>), grid, block, lds, st, logits, a);
-    else hipLaunchKernelGGL((route_kernel<16, BIAS, L>), grid, block, lds, st, logits, a);
+static int launch_route(const L* logits, RouteArgs a, hipStream_t st) {
+    for (int64_t left = a.tokens; left > 0; left -= ROUTE_AT_ONCE) {
+        a.tokens = std::min(left, ROUTE_AT_ONCE);
+        // one wave a workgroup where that still leaves CUs without one, else four
+        const int waves = a.tokens <= 512 ? 1 : 4;
+        const dim3 grid((unsigned)((a.tokens + waves - 1) / waves)), block(64 * waves);
+        const size_t lds = a.groups > 1 ? (size_t)waves * a.experts * sizeof(double) : 0;
+        const int epl = (a.experts + 63) / 64;
+        if (epl <= 1) hipLaunchKernelGGL((route_kernel<1, BIAS, L>), grid, block, lds, st, logits, a);
+        else if (epl <= 2) hipLaunchKernelGGL((route_kernel<2, BIAS, L>), grid, block, lds, st, logits, a);
+        else if (epl <= 4) hipLaunchKernelGGL((route_kernel<4, BIAS, L>), grid, block, lds, st, logits, a);
+        else if (epl <= 8) hipLaunchKernelGGL((route_kernel<8, BIAS, L>), grid, block, lds, st, logits, a);
+        else hipLaunchKernelGGL((route_kernel<16, BIAS, L>), grid, block, lds, st, logits, a);
+        if (const int rc = check_launch("route_experts")) return rc;
+        logits += a.tokens * a.experts;
+        a.weights += a.tokens * a.top_k;
+        a.ids += a.tokens * a.top_k;
+    }
+    return INT4MM_OK;
 }
 
 }  // namespace i4
@@ -246,10 +256,8 @@ extern "C" int int4mm_route_experts(void* weights, void* ids, const void* logits
     hipStream_t st = (hipStream_t)stream;
     if (sh->logits_bytes == 2) {
         const h16* l = static_cast<const h16*>(logits);
-        if (bias) launch_route<true>(l, a, st); else launch_route<false>(l, a, st);
-    } else {
-        const float* l = static_cast<const float*>(logits);
-        if (bias) launch_route<true>(l, a, st); else launch_route<false>(l, a, st);
+        return bias ? launch_route<true>(l, a, st) : launch_route<false>(l, a, st);
     }
-    return check_launch("route_experts");
+    const float* l = static_cast<const float*>(logits);
+    return bias ? launch_route<true>(l, a, st) : launch_route<false>(l, a, st);
 }

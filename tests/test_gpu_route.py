@@ -203,3 +203,13 @@ def test_refusals(ext):
 def test_a_bias_that_asks_for_a_gradient_is_refused(ext):
     with pytest.raises(RuntimeError, match="no backward"):
         ext.route_experts(logits_of(4, 32, torch.float16, 5), 2, bias=torch.zeros(32, device="cuda", requires_grad=True))
+
+
+def test_more_tokens_than_a_grid_has(ext):
+    """2^26 and a few tokens, 64 work-items for each: more than one launch holds"""
+    T, gen = 2 ** 26 + 5, torch.Generator(device="cuda").manual_seed(3)
+    logits = torch.empty((T, 2), dtype=torch.float16, device="cuda").normal_(generator=gen)
+    weights, ids = ext.route_experts(logits, 1, renormalize=False)
+    assert torch.equal(ids[:, 0], (logits[:, 1] > logits[:, 0]).to(torch.int32))
+    want = torch.sigmoid((logits[:, 1].double() - logits[:, 0].double()).abs())
+    assert ((weights[:, 0].double() - want).abs() <= WEIGHT_TOL * want).all()
