@@ -30,6 +30,14 @@ class LowRankAdapters(torch.nn.Module):
         self.register_buffer("up", torch.zeros((n_adapters, rank, out_features), dtype=torch.float16, device=device))
         self.register_buffer("scales", torch.zeros((n_adapters,), dtype=torch.float32, device=device))
 
+    def _apply(self, fn, recurse=True):
+        # half() and the like turn the factors alone: the scales are fp32 in every model
+        scales = self.scales
+        super()._apply(fn, recurse)
+        if self.scales.dtype != torch.float32:
+            self.scales = scales.to(self.scales.device)
+        return self
+
     @torch.no_grad()
     def set_adapter(self, index: int, down: torch.Tensor, up: torch.Tensor, scale: float = 1.0) -> None:
         """fills one adapter from its factors ``down`` ``[rank, in_features]`` and ``up`` ``[out_features, rank]``, of this rank or a lower one"""

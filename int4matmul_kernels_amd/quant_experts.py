@@ -44,6 +44,14 @@ class ExpertRouter(torch.nn.Module):
         self.topk_groups, self.group_score, self.renormalize, self.scale = topk_groups, group_score, renormalize, scale
         self.register_buffer("bias", torch.zeros((n_experts,), dtype=torch.float32, device=device) if bias else None)
 
+    def _apply(self, fn, recurse=True):
+        # half() and the like leave the bias alone: it is fp32 in every model
+        bias = self.bias
+        super()._apply(fn, recurse)
+        if bias is not None and self.bias.dtype != torch.float32:
+            self.bias = bias.to(self.bias.device)
+        return self
+
     def forward(self, logits: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         if logits.shape[-1] != self.n_experts:
             raise ValueError(f"logits must be [..., {self.n_experts}] but are {tuple(logits.shape)}")

@@ -139,3 +139,19 @@ def test_experts_grids():
     for T, k, E, K, F in ((4096, 8, 64, 2048, 1024), (8192, 2, 8, 4096, 14336), (32768, 8, 256, 7168, 2048), (2048, 4, 16, 4096, 32768)):
         code, size = call(T, k, E, K, F, 128)
         assert code == 6 and T * k * (2 * F + 4 * K) < size < 1.02 * T * k * (2 * F + 4 * K + 8) + 2 ** 20
+
+
+def test_half_leaves_fp32_buffers():
+    """a model turned to fp16 keeps the scales of its adapters and the bias of its router"""
+    router, adapters = ExpertRouter(8, 2, bias=True, device="cpu"), LowRankAdapters(3, 4, 64, 64, device="cpu")
+    router.bias.copy_(torch.linspace(-1, 1, 8) / 3)
+    adapters.scales.copy_(torch.tensor([1 / 3, 1e-9, 1e9]))
+    bias, scales = router.bias.clone(), adapters.scales.clone()
+    model = torch.nn.Sequential(router, adapters, ExpertRouter(8, 2, device="cpu"))
+    for turned in (model.half(), model.to(torch.float16), model.to("cpu", torch.float16), model.cpu()):
+        assert turned is model and turned[0] is router and turned[1] is adapters
+        assert router.bias.dtype == adapters.scales.dtype == torch.float32
+        assert torch.equal(router.bias, bias) and torch.equal(adapters.scales, scales)
+        assert adapters.down.dtype == adapters.up.dtype == torch.float16
+    assert set(model.state_dict()) == {"0.bias", "1.down", "1.up", "1.scales"}
+    assert model.to("meta")[1].scales.is_meta and model[0].bias.dtype == torch.float32
