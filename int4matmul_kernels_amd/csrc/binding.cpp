@@ -368,6 +368,7 @@ torch::Tensor low_rank_add(const torch::Tensor& base, const torch::Tensor& x, co
     torch::Tensor to;
     if (outs.has_value() && outs->defined()) {
         check_tensor(*outs, "outs", torch::kHalf, dev);
+        no_gradient({&*outs}, "low_rank_add");
         TORCH_CHECK(outs->sizes() == base.sizes(), "outs must be ", base.sizes());
         at::assert_no_partial_overlap(*outs, from);
         for (const auto* t : {&states, &down, &up, &scales, &ids}) at::assert_no_overlap(*outs, *t);

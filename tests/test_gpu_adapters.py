@@ -350,3 +350,15 @@ def test_prompts_of_many_rows(ext, rank, shape, n):
     base = p["base"].clone()
     ext.low_rank_add(base, p["x"], p["down"], p["up"], p["scales"], p["ids"], base)
     assert torch.equal(base, got)
+
+
+def test_outs_that_ask_for_a_gradient_are_refused(ext):
+    p = problem((4, 2), 3, 16)
+    outs = torch.zeros_like(p["base"]).requires_grad_()
+    for o in (outs, outs * 1):
+        with pytest.raises(RuntimeError, match="no backward"):
+            ext.low_rank_add(p["base"], p["x"], p["down"], p["up"], p["scales"], p["ids"], outs=o)
+    assert not outs.any()
+    with torch.no_grad():
+        ext.low_rank_add(p["base"], p["x"], p["down"], p["up"], p["scales"], p["ids"], outs=outs)
+    assert torch.equal(outs, add(ext, p))
