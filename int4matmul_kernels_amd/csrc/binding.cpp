@@ -388,6 +388,8 @@ torch::Tensor low_rank_add(const torch::Tensor& base, const torch::Tensor& x, co
                                  which.data_ptr(), &sh, ws.data_ptr(), (size_t)ws.numel(),
                                  (void*)c10::hip::getCurrentHIPStream(dev.index()).stream()),
              "low_rank_add");
+    // (a backward pass that has kept outs as it was has to notice)
+    if (outs.has_value() && !to.is_inference()) to.unsafeGetTensorImpl()->bump_version();
     return to;
 }
 

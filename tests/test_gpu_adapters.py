@@ -362,3 +362,17 @@ def test_outs_that_ask_for_a_gradient_are_refused(ext):
     with torch.no_grad():
         ext.low_rank_add(p["base"], p["x"], p["down"], p["up"], p["scales"], p["ids"], outs=outs)
     assert torch.equal(outs, add(ext, p))
+
+
+def test_outs_that_a_backward_pass_has_kept(ext):
+    """writing into a tensor that autograd keeps for a gradient: the backward pass refuses, as after torch's own in-place operations"""
+    p = problem((4, 2), 3, 16)
+    outs, w = p["base"].clone(), torch.ones(1, dtype=torch.float16, device="cuda", requires_grad=True)
+    loss = (outs * w).sum()
+    ext.low_rank_add(p["base"], p["x"], p["down"], p["up"], p["scales"], p["ids"], outs=outs)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        kept = torch.empty_like(outs)
+        ext.low_rank_add(p["base"], p["x"], p["down"], p["up"], p["scales"], p["ids"], outs=kept)
+    assert torch.equal(kept, outs)
