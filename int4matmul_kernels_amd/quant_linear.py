@@ -107,6 +107,8 @@ class QuantLinear(torch.nn.Module):
         ``adapter_ids`` (int32) are ``x``'s leading sizes, one or more of them"""
         if (adapters is None) != (adapter_ids is None):
             raise ValueError("adapters and adapter_ids come together")
+        if adapters is not None and x.is_floating_point():
+            x = x.contiguous().to(torch.float16)        # (once, for the projection and the adapters)
         # (the buffers straight from their dict: nn.Module's attribute look-up takes 0.3 us for each of the five)
         b = self._buffers
         try:

@@ -376,3 +376,28 @@ def test_outs_that_a_backward_pass_has_kept(ext):
         kept = torch.empty_like(outs)
         ext.low_rank_add(p["base"], p["x"], p["down"], p["up"], p["scales"], p["ids"], outs=kept)
     assert torch.equal(kept, outs)
+
+
+@pytest.mark.parametrize("dtype,apart,copies", [(torch.float16, False, 0), (torch.float32, False, 1), (torch.bfloat16, False, 1), (torch.float16, True, 1)])
+def test_states_are_converted_once(dtype, apart, copies):
+    """a layer with its adapters makes one fp16 copy of states that are not fp16 and contiguous"""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from int4matmul_kernels_amd.adapters import LowRankAdapters
+    from int4matmul_kernels_amd.quant_linear import QuantLinear
+
+    class Copies(TorchDispatchMode):
+        seen = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen += func.name() in ("aten::_to_copy", "aten::clone")
+            return func(*args, **(kwargs or {}))
+
+    torch.manual_seed(2)
+    layer, adapters = QuantLinear.from_float((torch.randn((128, 64), device="cuda") * 0.05).half(), 4, 64), LowRankAdapters(2, 4, 128, 64)
+    adapters.set_adapter(0, torch.randn((4, 128), device="cuda").half() * 0.1, torch.randn((64, 4), device="cuda").half())
+    ids = torch.tensor([0, -1, 0], dtype=torch.int32, device="cuda")
+    for shape in ((3, 128), (3, 5, 128)):
+        x = torch.randn((*shape[:-1], 256), device="cuda").to(dtype)[..., ::2] if apart else torch.randn(shape, device="cuda").to(dtype)
+        with Copies() as mode:
+            got = layer(x, adapters, ids)
+        assert torch.equal(got, layer(x.half().contiguous(), adapters, ids)) and mode.seen == copies
