@@ -395,3 +395,25 @@ def test_more_work_items_than_a_grid_has(ext):
                                              C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
     for rows in (slice(0, 4), slice(254, 258), slice(T // 2, T // 2 + 4), slice(T - 4, T)):
         close(outs[rows], plain(dict(p, x=p["x"][rows], ids=p["ids"][rows], weights=p["weights"][rows])))
+
+
+@pytest.mark.parametrize("T,n", [(32767, 3), (17000, 4096)])
+def test_a_share_beyond_32_bits(ext, T, n):
+    """pairs' results in one share of the workspace that are more than 2^32 elements apart, through the tiles and through the blocks of few pairs (of
+    whose 4096 experts the first three are asked, and only they are in memory)"""
+    import ctypes as C
+    from int4matmul_kernels_amd import capi
+    K, F, k = 32768, 64, 8
+    p, gen = problem(2, False, 3, 1, 1, K, F, 1024, seed=5), torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn((T, K), generator=gen, device="cuda").half()
+    ids = torch.randint(0, 3, (T, k), generator=gen, device="cuda").to(torch.int32)
+    weights = torch.rand((T, k), generator=gen, device="cuda")
+    sh = capi.experts_shape(T, k, n, K, F, 1024)
+    size = capi.lib().int4mm_experts_workspace_bytes(C.byref(sh))
+    assert T * k * K > 2 ** 32 and size > 4 * T * k * K                       # (all of them at once)
+    ws, outs = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.empty((T, K), dtype=torch.float16, device="cuda")
+    ptr = lambda t: C.c_void_p(None if t is None else t.data_ptr())
+    assert capi.lib().int4mm_experts_forward(2, *map(ptr, (outs, x, weights, ids, *p["up"], *p["down"])), C.byref(sh), ptr(ws), size,
+                                             C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    for rows in (slice(0, 30), slice(T // 2, T // 2 + 30), slice(T - 30, T)):
+        close(outs[rows], plain(dict(p, x=x[rows], ids=ids[rows], weights=weights[rows])))
