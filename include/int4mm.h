@@ -287,7 +287,7 @@ INT4MM_API int int4mm_route_experts(void* weights, void* ids, const void* logits
  * hold a packed matrix of in_size K, out_size 2 F and one of F, K per expert in the formats above, scales and zeros [E, groups, 2 F]
  * and [E, groups, K], masks (16:32: both, else NULL) [E, K / 32, 2 F] and [E, F / 32, K].  A pair whose id is outside 0 ... E - 1
  * adds nothing (its weight is not looked at); a token without a pair gets 0.  The same expert may be named twice.  Sums are fp32;
- * up to 40 pairs an expert, if all are asked alike, exact codes are multiplied (16:32: codes less their zero, rounded once) and
+ * up to 48 pairs an expert, if all are asked alike, exact codes are multiplied (16:32: codes less their zero, rounded once) and
  * scale and zero applied to the sums, beyond that int4mm_dequantize's weights.  Results are a deterministic function of the arguments.
  * K and F multiples of 64 below 2^24, K F < 2^31, at most 4096 experts and 1024 slots a token (fewer where K or F is beyond a million: a grid
  * has fewer than 2^32 work-items, 512 for a pair and 64 columns).  The workspace holds what up to 2^18 pairs at a time need; more go

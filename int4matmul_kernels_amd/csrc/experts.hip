@@ -630,12 +630,17 @@ __global__ __launch_bounds__(256) void combine_kernel(h16* outs, const float* pa
 //
 // A pair by itself: one token, or so few pairs that hardly two of them share an expert.
 //
-// Blocks of rows_kernel up to a mean of 40, then tiles.  us a call, 16 experts of 2048 x 1408, means of 32 / 48 / 64 / 96: blocks int4 43 /
-// 54 / 63 / 84, int3 49 / 62 / 72 / 97, int2 46 / 58 / 67 / 90, 16:32 60 / 72 / 86 / 116; tiles int4 - / 53 / 56 / 63, int3 - / 58 / 60 / 65, int2 - /
-// 52 / 55 / 59, 16:32 - / 77 / 79 / 85.
+// Blocks of rows_kernel up to a mean of 48, then tiles.  us a call, blocks / tiles:
+//   16 experts of 2048 x 1408, mean 32    int4 45 / 56     int3 46 / 58     int2 44 / 52     16:32 58 / 78
+//                                   48         51 / 54          60 / 59          57 / 53           73 / 77
+//                                   64         61 / 56          71 / 62          67 / 55           85 / 80
+//   8 experts of 4096 x 11008,      40         256 / 317        293 / 340        267 / 294         349 / 420
+//                                   48         276 / 319        309 / 340        280 / 295         364 / 420
+//                                   64         335 / 323        381 / 346        341 / 302         446 / 433
 //
 // The height of the tiles, for each product: a tile of up to 64 / 96 / 128 / 192 / 256 rows takes 8 us and, on a full grid, 0.43 / 0.47 / 0.53 / 0.69 /
 // 0.86 a K step; the tiles are those of experts that are asked unevenly, with a deviation of half the mean beside that of independent choices.
+constexpr int BLOCKS_UP_TO = 48;
 struct ExpertsPlan { bool single, tiles; int up, down; };          // up, down: heights of the tiles
 static double tiles_us(double mean, int experts, int height, int64_t strips, int64_t steps) {
     // (the middles of eight equal parts of the normal distribution)
@@ -656,7 +661,7 @@ static double tiles_us(double mean, int experts, int height, int64_t strips, int
 static ExpertsPlan plan_experts(const int4mm_experts_shape& sh) {
     const int64_t pairs = sh.tokens * sh.top_k, K = sh.in_size, F = sh.width;
     const double mean = (double)pairs / sh.experts;
-    ExpertsPlan p{pairs <= 64 && (sh.tokens == 1 || 2 * pairs <= sh.experts), mean > 40, 128, 128};
+    ExpertsPlan p{pairs <= 64 && (sh.tokens == 1 || 2 * pairs <= sh.experts), mean > BLOCKS_UP_TO, 128, 128};
     if (p.single || !p.tiles) return p;
     // (`row`: of the second product, whose tiles address their rows with 31 bits; 64 rows of any width that check_experts admits)
     auto height = [&](int64_t strips, int64_t steps, int64_t row) {
@@ -705,10 +710,10 @@ static int64_t work_items(const int4mm_experts_shape& sh) {
 constexpr int64_t PAIRS_AT_ONCE = (int64_t)1 << 18, GRID_ITEMS = ((int64_t)1 << 32) - 4096;
 static int64_t tokens_at_once(const int4mm_experts_shape& sh) {
     int64_t most = std::max<int64_t>(1, std::min((((int64_t)1 << 31) - 1) / (2 * sh.in_size), PAIRS_AT_ONCE / sh.top_k));
-    // (the most that any number of pairs takes: blocks up to a mean of 40, the lowest tiles, 64 pairs by themselves; a pair never takes
+    // (the most that any number of pairs takes: blocks up to their mean, the lowest tiles, 64 pairs by themselves; a pair never takes
     // more than 512 work-items a strip)
     const int64_t E = sh.experts, strips = std::max(sh.in_size, 2 * sh.width) / 64;
-    if ((E + std::min(PAIRS_AT_ONCE, 40 * E) / ROWS_HEIGHT) * strips * (64 * ROWS_WAVES) > GRID_ITEMS ||
+    if ((E + std::min(PAIRS_AT_ONCE, BLOCKS_UP_TO * E) / ROWS_HEIGHT) * strips * (64 * ROWS_WAVES) > GRID_ITEMS ||
         (E + PAIRS_AT_ONCE / 64) * ((strips + 3) / 4) * 512 > GRID_ITEMS || 64 * strips * 512 > GRID_ITEMS)
         most = std::min(most, std::max<int64_t>(1, GRID_ITEMS / (strips * 512) / sh.top_k));
     const int64_t shares = (sh.tokens + most - 1) / most;
