@@ -268,7 +268,7 @@ INT4MM_API int int4mm_dequantize(int bits, void* w_out, const void* matrix, cons
  *   key = logits without a bias, p + bias with one (NaN or -inf: out); the top_k largest keys, ties to the lowest expert
  *   groups > 1: only experts of the topk_groups best groups of experts / groups neighbours, by their best key (group_score 0)
  *   or the sum of their two best p (p + bias with a bias; 1), ties to the lowest group
- *   weights = p, divided by their sum if `renormalize`, times `scale`
+ *   weights = p, divided by their sum if `renormalize` (a sum of 0, where every p is below what 64 bits hold, stays 0), times `scale`
  * p, keys and sums are held in 64 bits, weights rounded once.  Where fewer than top_k experts are left the last slots have
  * id -1 and weight 0.  experts <= 1024, top_k <= 64, groups <= 64; top_k <= experts / groups * topk_groups. */
 typedef struct int4mm_route_shape {
@@ -310,7 +310,8 @@ INT4MM_API int int4mm_experts_forward(int bits, void* outs, const void* x, const
  *   outs[t,:] = fp16( base[t,:] + scales[a] * (x[t,:] @ down[a]^T) @ up[a] ),   a = ids[t / rows_per_id]
  * x fp16 [rows, K], base and outs fp16 [rows, S] (outs may be base), down fp16 [adapters, rank, K], up fp16 [adapters, rank, S], scales
  * fp32 [adapters], ids int32 [ceil(rows / rows_per_id)].  A row whose id is outside 0 ... adapters - 1 keeps its base.  An
- * adapter of a lower rank has zeros in its last ranks.  K and S multiples of 64, rank 1 ... 512, rows up to 1048560. */
+ * adapter of a lower rank has zeros in its last ranks.  K and S multiples of 64, rank 1 ... 512, rows up to 1048560.  x @ down^T is multiplied as
+ * two parts of 11 bits each, so that an infinity of `up` may come out as NaN in the rows that use it. */
 typedef struct int4mm_adapter_shape {
     int64_t rows, rows_per_id, adapters, rank;
     int64_t in_size;       /* K */

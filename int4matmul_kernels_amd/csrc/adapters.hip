@@ -373,6 +373,8 @@ __global__ __launch_bounds__(256) void expand_kernel(AdapterArgs a) {
 // Rows ordered by adapter or not: ids per row, adapters, rank, K, S: 256, 16, 16, 5120, 5120 13.2 / 20.8; 256, 128, 16, 5120, 5120 23.1 / 23.8; 777,
 // 24, 20, 2048, 1408 15.5 / 24.2; 777, 4, 16, 2048, 1408 13.5 / 12.6; 1500, 128, 16, 5120, 5120 26 / 125; 4096, 2, 16, 5120, 5120 43 / 45; 4096, 100,
 // 64, 4096, 4096 84 / 473; where it does not gain, 128, 128, 16, 4096, 4096 16.7 / 13.0; one row 11.9 / 8.4.
+// Only rows with an id each, up to 256 adapters and 65536 rows (the order reads all ids for every adapter) whose states and outputs are addressed with 31
+// bits: beyond that a tile goes through all of its adapters, however many those are.
 constexpr double SORTED_GAIN = 2.0;                   // tiles times their adapters over tiles of one adapter
 struct AdapterPlan { int mt, nt, ksplit, units_per_split, deal_shrink, deal_expand, strips; bool sorted; int64_t tiles; };
 

@@ -7,9 +7,9 @@
 // the 256 registers that a lane has.  A pair's result is stored in fp32, as those of rows_kernel are: its weight, which may be what brings it into
 // fp16's range, comes after it.  (In fp16 calls took 2 - 12 % less, 16:32 experts gaining most, and a result beyond 65504 was lost.)
 //
-// What bounds it: large batches the power limit (4096 tokens, eight of 64 experts of 2048 x 1024, int4: 282 and 164 us for 275 and 137 GFLOP, tiles' rows beyond
-// an expert's last one included 1.1 PFLOP/s); few rows the chain of a step, 0.44 us whatever the height.  One height for all of a launch's blocks instead: 510 us a
-// call where this takes 466.
+// What bounds it: large batches the beginnings and ends of tiles, 8 us beside 55 and 27 in the steps, and then the power limit (4096 tokens, eight of 64 experts
+// of 2048 x 1024, int4: 336 and 214 us for 275 and 137 GFLOP, matrix pipe busy 49 and 35 %); few rows the chain of a step, 0.44 us whatever the height.  One
+// height for all of a launch's blocks instead: 510 us a call where blocks of their own took 466.
 #include "experts.h"
 
 #include <algorithm>
