@@ -23,6 +23,9 @@
 // issue of the fold and the decode and the ends of the workgroups.  Three units in flight are slower (192: registers), so are strips that are
 // neighbours on an XCD (193), and non-temporal loads where the weights fit the last-level cache (37 / 42, 16 experts of 2048 x 1408,
 // 16 pairs each).
+// Both heights share a kernel, whose registers are those of the two row tiles.  Compiled with one row tile alone, blocks of 16 pairs, it takes int4 43,
+// int3 54 - 60, int2 51, 16:32 66 - 72 where this takes 53, 68, 58 - 63, 84 (64 experts of 2048 x 1024, 2 pairs each), at means of 8 to 16 the two cross, and
+// at 32 it loses a fifth (8 experts of 4096 x 11008, int4 259 / 210): a kernel of its own for small means is left to do.
 #include "experts.h"
 
 #include <algorithm>
