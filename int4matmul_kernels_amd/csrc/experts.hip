@@ -16,7 +16,7 @@
 // (sum x w = s (sum x q - z sum x), the sum of x from a product with ones), which takes 7 instructions a word where rounded weights
 // take 17 and is nearer to the exact product.  The partial sums of the waves meet in LDS.
 //
-// Measured (64 tokens, two of eight experts of 4096 x 11008, int4, us a call on one box): weights rounded, addresses computed, one lane
+// Measured (64 tokens, two of eight experts of 4096 x 11008, int4, us a call on one GPU): weights rounded, addresses computed, one lane
 // for 16 bytes of every row of states 198; exact codes, buffer loads, two units in flight in the order that the waits go by 178; states
 // read row by row and turned in LDS 172; states straight to LDS, blocks of up to 16 pairs with one row tile 155 - 166.  With all
 // weights from cache 129 before the last step, without the fold of the groups' sums 107: not the bytes, the
